@@ -202,13 +202,6 @@ SHDW_DEVICE void fetch(const char* from, char* to, int wave, int lane) {
 // by up to kLag, and down to 2^-34 of the largest before fp16 rounds them away.
 constexpr float kLift = 10.f, kLag = 5.f;
 
-// Waits for all loads where the compiler sees it, so that it does not wait where a rare path joins the others: there it would be
-// for the copies that are under way.
-SHDW_DEVICE void loads_done() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0);
-}
-
 // The tiles that go through fp32 operands are rare and their code is long: functions of their own, so that the
 // others' registers do not depend on them.
 // Scores of a tile with the rows' operands q [2 NB][hi, lo].

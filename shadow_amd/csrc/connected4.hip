@@ -30,6 +30,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/shadow_hip.h"
 #include "device_common.h"
@@ -531,6 +532,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void connected4_few_kernel(const
 constexpr int kManyRows = 128, kManyOut = 128;  // of a workgroup
 constexpr int kStageWords = 8;                  // 64 codes
 constexpr uint32_t kStageBytes = 2 * 32 * kStageWords * 16;  // of 32 rows: hi, lo
+constexpr int kStageSums = 128;                 // of 32 rows: sums and factors of two groups
 constexpr int kSplitRows = 8, kSplitParts = 4;
 
 // Words of a stage in the order of the four products: words 0 1 4 5 in lanes 0..31, 2 3 6 7 in lanes 32..63.
@@ -538,10 +540,16 @@ SHDW_DEVICE int stage_lane(int word, int row) { return (word & 2) * 16 + row; }
 SHDW_DEVICE int stage_product(int word) { return (word >> 2) * 2 + (word & 1); }
 
 // x in the order that the lanes of the products take it: [32 rows][stage][hi, lo][product][lane], and of every
-// stage and row the sums over groups that start there, [32 rows][stage][2][32].  A workgroup takes eight rows and
-// a part of `in`, after the largest value of the rows, which gives their power of two.
+// stage and row the sums over groups that start there, [32 rows][stage][2][32], and behind these, [2][32], what takes a group's
+// products to the row's units.  A workgroup takes eight rows and a part of `in`, after the largest value of the rows, which gives
+// their power of two.  A group whose largest value is less than 2^-8 of the row's has a power of its own, undone before its
+// steps: in the row's it would be held to 2^-34 of the row's largest value (odd codes' numbers are 2^4 smaller), which shows where
+// that one meets small weights.  Other groups share the row's and need no factor; `apart`, a word for every
+// workgroup, says whether any has its own.
+constexpr float kNear = 0x1p-8f;
+constexpr int kMostLift = 120;  // of a group above its row: 2^-kMostLift is normal
 template <int GROUP_WORDS, bool LOWS>
-__global__ __launch_bounds__(kBlock) void connected4_split_kernel(const float* x, v8h* parts, float* sums, float* undo,
+__global__ __launch_bounds__(kBlock) void connected4_split_kernel(const float* x, v8h* parts, float* sums, float* undo, uint32_t* apart,
                                                                   uint32_t rows, uint32_t words, uint32_t stages) {
   const int lane = threadIdx.x % 32, sub = threadIdx.x / 32;  // 32 lanes a row
   const uint32_t row = blockIdx.x * kSplitRows + sub;
@@ -565,6 +573,7 @@ __global__ __launch_bounds__(kBlock) void connected4_split_kernel(const float* x
   const uint32_t turns = (stages + 3) / 4;  // of 32 words: four stages, whole groups
   const uint32_t from = turns * blockIdx.y / kSplitParts, to = turns * (blockIdx.y + 1) / kSplitParts;
   const uint32_t block = row / 32, r = row % 32;
+  bool own = false;
   for (uint32_t turn = from; turn < to; turn += kTurns) {
     float all[kTurns][8];
 #pragma unroll
@@ -580,45 +589,63 @@ __global__ __launch_bounds__(kBlock) void connected4_split_kernel(const float* x
         v[c] = real ? all[n][c] : 0.f;
         sum += v[c];
       }
+      float group_most = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) group_most = larger(group_most, __builtin_fabsf(v[c]));
       sum = across_lanes<GROUP_WORDS>(sum, [](float a, float b) { return a + b; });
+      group_most = across_lanes<GROUP_WORDS>(group_most, [](float a, float b) { return larger(a, b); });
       if (stage >= stages) continue;
+      const int lift = group_most == 0.f || group_most >= most * kNear ? e : min(lift_of(group_most), e + kMostLift);
+      own = own || lift != e;
       const int word = w % kStageWords;
       v8h hi, lo;
-      operand_of(v, power2(e), hi, lo);
+      operand_of(v, power2(lift), hi, lo);
       v8h* out = parts + (static_cast<uint64_t>(block) * stages + stage) * (kStageBytes / 16) + stage_product(word) * kWave +
                  stage_lane(word, r);
       out[0] = hi;
       out[kStageBytes / 32] = lo;
-      // in the units of the products
-      if (w % GROUP_WORDS == 0)
-        sums[((static_cast<uint64_t>(block) * stages + stage) * 2 + word / 4) * 32 + r] =
-            sum * power2(e) * (LOWS ? 1.f : -8.f);
+      // in the units of the products, where they are added to them, else in the row's
+      float* const group = sums + (static_cast<uint64_t>(block) * stages + stage) * kStageSums + word / 4 * 32 + r;
+      if (w % GROUP_WORDS == 0) group[0] = LOWS ? sum * power2(e) : sum * power2(lift) * -8.f;
+      if (w % min(GROUP_WORDS, kStageWords) == 0) group[64] = power2(e - lift);
     }
   }
+  const int any = __syncthreads_or(own);
+  if (threadIdx.x == 0) apart[blockIdx.x * kSplitParts + blockIdx.y] = any;
 }
 
 // What a workgroup has of a stage in LDS, all of it copied there without a register in between: x and its sums of
 // four blocks of 32 rows; codes, steps and lows of four blocks of 32 outputs.
 struct alignas(16) ManyStage {
   char x[4][kStageBytes];
-  float sums[4][64];
+  float sums[4][kStageSums];
   v4u codes[4][32][2];  // [output][half a row]
   float steps[4][64], lows[4][64];  // [group of the stage][output]
 };
 constexpr int kManyBuffers = 3;
 
-// p[0] and p[64] of what to_lds4 copied.  Read by an instruction of our own, waited for at once: in front of a read that it
-// sees to alias such a copy the compiler waits for all copies that are under way, two stages of them.
+// p[0] and p[64], and four each from p, p + 8, p + 16 and p + 24 on, of what was copied to LDS.  Read by instructions of our own,
+// waited for at once: in front of a read that it sees to alias such a copy the compiler waits for all copies that are under
+// way, two stages of them.
+SHDW_DEVICE uint32_t lds_address(const float* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const float*)p));
+}
 SHDW_DEVICE v2f lds_pair(const float* p) {
-  const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const float*)p));
   v2f v;
-  asm volatile("ds_read2_b32 %0, %1 offset0:0 offset1:64\n\ts_waitcnt lgkmcnt(0)" : "=v"(v) : "v"(at) : "memory");
+  asm volatile("ds_read2_b32 %0, %1 offset0:0 offset1:64\n\ts_waitcnt lgkmcnt(0)" : "=v"(v) : "v"(lds_address(p)) : "memory");
   return v;
+}
+SHDW_DEVICE v16f lds_rows(const float* p) {
+  v4f a, b, c, d;
+  asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:32\n\tds_read_b128 %2, %4 offset:64\n\t"
+               "ds_read_b128 %3, %4 offset:96\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d) : "v"(lds_address(p)) : "memory");
+  return v16f{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3], c[0], c[1], c[2], c[3], d[0], d[1], d[2], d[3]};
 }
 
 template <int GROUP_WORDS, bool LOWS>
 __global__ __launch_bounds__(kBlock, 1) void connected4_many_kernel(const v8h* parts, const float* sums, const float* undo,
-                                                                    const uint32_t* codes, float* y, float* partial,
+                                                                    const uint32_t* apart, const uint32_t* codes, float* y, float* partial,
                                                                     uint32_t stages, uint32_t splits, uint32_t row_tiles,
                                                                     Connected4Args p) {
   __shared__ ManyStage lds[kManyBuffers];
@@ -633,15 +660,15 @@ __global__ __launch_bounds__(kBlock, 1) void connected4_many_kernel(const v8h* p
   const uint64_t my_codes = static_cast<uint64_t>(min(first_out + lane / 2, p.out - 1)) * p.words;
   const uint64_t my_groups = static_cast<uint64_t>(min(first_out + lane % 32, p.out - 1)) * p.groups;
   const char* const my_x = reinterpret_cast<const char*>(parts) + static_cast<uint64_t>(row_tile * 4 + wave) * stages * kStageBytes + lane * 16;
-  const float* const my_sums = sums + static_cast<uint64_t>(row_tile * 4 + wave) * stages * 64 + lane % 16 * 4;
+  const float* const my_sums = sums + static_cast<uint64_t>(row_tile * 4 + wave) * stages * kStageSums + lane % 32 * 4;
   constexpr int kStageGroups = GROUP_WORDS == 4 ? 2 : 1;
   constexpr int kCopies = static_cast<int>(kStageBytes / 1024) + 3 + (LOWS ? 1 : 0);  // of a wave and stage, at least
-  const auto fetch = [&](uint32_t stage) {
+  const auto fetch = [&](uint32_t stage, bool factors) {
     ManyStage& to_stage = lds[(stage - from) % kManyBuffers];
 #pragma unroll
     for (int n = 0; n < static_cast<int>(kStageBytes / 1024); ++n)
       to_lds16(my_x + static_cast<uint64_t>(stage) * kStageBytes + n * 1024, to_stage.x[wave] + n * 1024);
-    if (lane < 16) to_lds16(my_sums + static_cast<uint64_t>(stage) * 64, to_stage.sums[wave]);
+    if (lane < (factors ? 32 : 16)) to_lds16(my_sums + static_cast<uint64_t>(stage) * kStageSums, to_stage.sums[wave]);
     if ((stage + 1) * kStageWords <= p.words) {
       to_lds16(codes + my_codes + stage * kStageWords + lane % 2 * 4, to_stage.codes[wave]);
     } else {
@@ -656,6 +683,9 @@ __global__ __launch_bounds__(kBlock, 1) void connected4_many_kernel(const v8h* p
     to_lds4(p.steps + my_groups + group, to_stage.steps[wave]);
     if (LOWS) to_lds4(p.lows + my_groups + group, to_stage.lows[wave]);
   };
+
+  static_assert(kManyRows / kSplitRows * kSplitParts == kWave, "a lane a word");
+  const uint64_t some = __builtin_amdgcn_ballot_w64(apart[row_tile * kWave + lane] != 0);
 
   v16f acc[2][2], run[2][2];  // [32 rows][32 outputs]
 #pragma unroll
@@ -699,7 +729,7 @@ __global__ __launch_bounds__(kBlock, 1) void connected4_many_kernel(const v8h* p
           for (int r = 0; r < 4; ++r) sum[m][u][4 * c + r] = q[r];
         }
   };
-  const auto work = [&](uint32_t stage, const Operands& k, bool opens, bool closes) {
+  const auto work = [&](uint32_t stage, const Operands& k, bool opens, bool closes, auto factors) {
     const ManyStage& here = lds[(stage - from) % kManyBuffers];
 #pragma unroll
     for (int u = 0; u < kStageGroups; ++u) {
@@ -716,6 +746,16 @@ __global__ __launch_bounds__(kBlock, 1) void connected4_many_kernel(const v8h* p
             run[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k.lo[m][t], k.codes[n][t], run[m][n], 0, 0, 0);
           }
       if (closes) {
+        if constexpr (factors) {
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const v16f f = lds_rows(&here.sums[wave_rows * 2 + m][64 + u * 32 + 4 * half]);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+#pragma unroll
+              for (int n = 0; n < 2; ++n) run[m][n][r] *= f[r];
+          }
+        }
         const v2f step = lds_pair(&here.steps[wave_out * 2][u * 32 + j]), low = LOWS ? lds_pair(&here.lows[wave_out * 2][u * 32 + j]) : step;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -731,21 +771,27 @@ __global__ __launch_bounds__(kBlock, 1) void connected4_many_kernel(const v8h* p
   };
   // two stages are on their way while one is worked on; `from` and `to` are even, a group of 128 is two stages
   constexpr bool kEvery = GROUP_WORDS < 16;  // stage has groups of its own
-  if (from < to) fetch(from), fetch(from + 1);
-  for (uint32_t stage = from; stage < to; stage += 2) {
-    copies_done<kCopies>();
-    if (stage + 2 < to) fetch(stage + 2);
-    Operands k;
-    read_sums(stage);
-    read(stage, k);
-    work(stage, k, true, kEvery);
-    if (stage + 2 < to) copies_done<kCopies>();
-    else copies_done<0>();
-    if (stage + 3 < to) fetch(stage + 3);
-    if (kEvery) read_sums(stage + 1);
-    read(stage + 1, k);
-    work(stage + 1, k, kEvery, true);
-  }
+  if (from < to) fetch(from, true), fetch(from + 1, true);
+  const auto all = [&](auto factors) {
+    for (uint32_t stage = from; stage < to; stage += 2) {
+      copies_done<kCopies>();
+      if (stage + 2 < to) fetch(stage + 2, factors);
+      Operands k;
+      read_sums(stage);
+      read(stage, k);
+      work(stage, k, true, kEvery, factors);
+      if (stage + 2 < to) copies_done<kCopies>();
+      else copies_done<0>();
+      if (stage + 3 < to) fetch(stage + 3, factors);
+      if (kEvery) read_sums(stage + 1);
+      read(stage + 1, k);
+      work(stage + 1, k, kEvery, true, factors);
+    }
+  };
+  // Factors of groups, where any of the 128 rows has one: a loop of its own, since looking for them in every group takes 6 % of
+  // 700 rows on 4096 x 4096 weights, 11 % with groups of 64.
+  if (some != 0) all(std::true_type());
+  else all(std::false_type());
   // everything is loaded in front of the first store: a load behind one waits for it
   v4f back[2][4];
   float bias[2];
@@ -760,7 +806,7 @@ __global__ __launch_bounds__(kBlock, 1) void connected4_many_kernel(const v8h* p
     out[n] = out_tile * kManyOut + wave_out * 64 + n * 32 + j;
     bias[n] = p.bias ? p.bias[min(out[n], p.out - 1)] : 0.f;
   }
-  asm volatile("" ::: "memory");
+  loads_done();  // or every store would wait for the one in front of it
   float* const to_y = splits > 1 ? partial + static_cast<uint64_t>(part) * p.rows * p.out : y;
   const bool with_bias = splits == 1 && p.bias;
 #pragma unroll
@@ -792,8 +838,8 @@ __global__ __launch_bounds__(kStream) void connected4_join_kernel(const float* p
 
 struct ManyPlan {
   uint32_t row_tiles, out_tiles, stages, splits;
-  size_t parts_bytes, sums_bytes, undo_bytes, partial_bytes;
-  size_t bytes() const { return parts_bytes + sums_bytes + undo_bytes + partial_bytes; }
+  size_t parts_bytes, sums_bytes, undo_bytes, apart_bytes, partial_bytes;
+  size_t bytes() const { return parts_bytes + sums_bytes + undo_bytes + apart_bytes + partial_bytes; }
 };
 // Which kernel, by what it costs: 16 rows at a time 4 us and 0.165 for a million weights and set of 16, tiles 15 us (two or three launches, few
 // of them whole on the chip) and 0.8 for a million weights and 128 rows.  4096 x 4096 weights: 128 rows 23.3 us by 16 and 29.0 in
@@ -813,8 +859,9 @@ static ManyPlan plan_many(int rows, int in, int out) {
   const uint64_t tiles = static_cast<uint64_t>(m.row_tiles) * m.out_tiles;
   m.splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(256 / tiles, m.stages / 8)));
   m.parts_bytes = static_cast<size_t>(m.row_tiles) * 4 * m.stages * kStageBytes;
-  m.sums_bytes = static_cast<size_t>(m.row_tiles) * 4 * m.stages * 64 * sizeof(float);
+  m.sums_bytes = static_cast<size_t>(m.row_tiles) * 4 * m.stages * kStageSums * sizeof(float);
   m.undo_bytes = static_cast<size_t>(m.row_tiles) * kManyRows * sizeof(float);
+  m.apart_bytes = static_cast<size_t>(m.row_tiles) * kWave * sizeof(uint32_t);
   m.partial_bytes = m.splits == 1 ? 0 : static_cast<size_t>(m.splits) * rows * out * sizeof(float);
   return m;
 }
@@ -826,12 +873,13 @@ static int launch_many(const ManyPlan& m, const float* x, const uint32_t* codes,
   v8h* parts = reinterpret_cast<v8h*>(at);
   float* sums = reinterpret_cast<float*>(at + m.parts_bytes);
   float* undo = reinterpret_cast<float*>(at + m.parts_bytes + m.sums_bytes);
-  float* partial = reinterpret_cast<float*>(at + m.parts_bytes + m.sums_bytes + m.undo_bytes);
+  uint32_t* apart = reinterpret_cast<uint32_t*>(at + m.parts_bytes + m.sums_bytes + m.undo_bytes);
+  float* partial = reinterpret_cast<float*>(at + m.parts_bytes + m.sums_bytes + m.undo_bytes + m.apart_bytes);
   const dim3 split_grid(m.row_tiles * kManyRows / kSplitRows, kSplitParts);
-  connected4_split_kernel<GROUP_WORDS, LOWS><<<split_grid, kBlock, 0, st>>>(x, parts, sums, undo, p.rows, p.words, m.stages);
+  connected4_split_kernel<GROUP_WORDS, LOWS><<<split_grid, kBlock, 0, st>>>(x, parts, sums, undo, apart, p.rows, p.words, m.stages);
   if (int rc = launch_status()) return rc;
   connected4_many_kernel<GROUP_WORDS, LOWS><<<m.row_tiles * m.out_tiles * m.splits, kBlock, 0, st>>>(
-      parts, sums, undo, codes, y, partial, m.stages, m.splits, m.row_tiles, p);
+      parts, sums, undo, apart, codes, y, partial, m.stages, m.splits, m.row_tiles, p);
   if (int rc = launch_status()) return rc;
   if (m.splits > 1) {
     const uint32_t count = p.rows * p.out;

@@ -57,6 +57,13 @@ SHDW_DEVICE void copies_done() {
   asm volatile("s_barrier" ::: "memory");
 }
 
+// Waits for all loads where the compiler sees it, so that it does not wait later, where a rare path joins the others or a store may
+// not be made: there it would be for copies or stores that are under way.
+SHDW_DEVICE void loads_done() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0);
+}
+
 }  // namespace shdw
 
 #endif  // SHADOW_AMD_CSRC_SPLIT16_H_
