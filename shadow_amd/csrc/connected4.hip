@@ -4,7 +4,9 @@
 // 8.  Without `lows` a group's low end is -8 steps.  The reference's fully connected operator has
 // fp32 weights only.
 //
-// A group's part of an output is step * sum(code * x) + low * sum(x), the sums on matrix instructions, the rest in fp32.
+// A group's part of an output is step * sum(code * x) + low * sum(x), the sums on matrix instructions, the rest in fp32.  Both
+// sums are in units of a power of two that x is scaled by, which is undone behind the step: in x's own units they would leave
+// fp32's range from |x| of 2^117 on, where x and the result are still within it.
 //
 // Up to 8 rows: the codes are read once and that is the time, and unpacking them what stands in its way.  x becomes
 // a whole number of 23 bits and a sign in units of a group's power of two, in three digits to the base 256; four rows' digits are
@@ -114,7 +116,8 @@ SHDW_DEVICE void few_place(int word, int& g, int& t) {
   }
 }
 
-// A lane's word of a row as digits, and its group's factor that undoes the power of two and sum (times -8 without lows).
+// A lane's word of a row as digits, and its group's factor that undoes the power of two and sum, in units of the last digit
+// (times -8 without lows).
 struct Digits {
   uint2 top, middle, low;  // eight digits each: of even codes, of odd ones
   float factor, sum;
@@ -123,9 +126,8 @@ template <int GROUP_WORDS, bool LOWS>
 SHDW_DEVICE Digits digits_of(const float (&v)[8]) {
   float most = 0.f, sum = 0.f;
 #pragma unroll
-  for (int c = 0; c < 8; ++c) most = larger_or_nan(most, __builtin_fabsf(v[c])), sum += v[c];
+  for (int c = 0; c < 8; ++c) most = larger_or_nan(most, __builtin_fabsf(v[c]));
   most = across_lanes<GROUP_WORDS>(most, [](float a, float b) { return larger_or_nan(a, b); });
-  sum = across_lanes<GROUP_WORDS>(sum, [](float a, float b) { return a + b; });
   // the largest in [2^22, 2^23) / 1.0045: three digits hold up to 127 * 65793 = 2^23 / 1.0039
   const int e = min(126, 22 - max(-104, exponent_of(most * 1.0045f)));
   const float f = power2(e);
@@ -133,7 +135,9 @@ SHDW_DEVICE Digits digits_of(const float (&v)[8]) {
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
     // v = 65536 a + 256 b + c, each in -128 .. 127
-    const int d = static_cast<int>(__builtin_rintf(v[c] * f));
+    const float scaled = v[c] * f;
+    sum += scaled;
+    const int d = static_cast<int>(__builtin_rintf(scaled));
     const int lo = static_cast<int8_t>(d), rest = (d - lo) >> 8, mid = static_cast<int8_t>(rest), hi = (rest - mid) >> 8;
     const int word = c % 2, byte = c / 2 * 8;  // even codes in one register, odd ones in the next
     top[word] |= static_cast<uint32_t>(hi & 255) << byte;
@@ -143,6 +147,7 @@ SHDW_DEVICE Digits digits_of(const float (&v)[8]) {
   Digits d;
   d.top = make_uint2(top[0], top[1]), d.middle = make_uint2(middle[0], middle[1]), d.low = make_uint2(low[0], low[1]);
   d.factor = most < INFINITY ? power2(-e) : NAN;  // digits hold nothing that is not finite
+  sum = across_lanes<GROUP_WORDS>(sum, [](float a, float b) { return a + b; });
   d.sum = LOWS ? sum : sum * -8.f;
   return d;
 }
@@ -181,12 +186,7 @@ SHDW_DEVICE void add_digits(v4u x0, v4u x1, const v4u (&b)[2], const float* fact
   const auto add = [&](int u, v4i d) {
     const float2 factor = *reinterpret_cast<const float2*>(factors + u * PITCH);
     const float f = __builtin_fmaf(static_cast<float>(d[0]), 65536.f, __builtin_fmaf(static_cast<float>(d[1]), 256.f, static_cast<float>(d[2])));
-    if (LOWS) {
-      sum = __builtin_fmaf(f * factor.x, step[u], sum);
-      sum = __builtin_fmaf(factor.y, low[u], sum);
-    } else {
-      sum = __builtin_fmaf(__builtin_fmaf(f, factor.x, factor.y), step[u], sum);
-    }
+    sum = __builtin_fmaf(LOWS ? __builtin_fmaf(factor.y, low[u], f * step[u]) : (f + factor.y) * step[u], factor.x, sum);
   };
   const v4u x[2] = {x0, x1};
   if (GROUP_WORDS == 4) {
@@ -273,7 +273,7 @@ struct DigitRows {
 };
 
 // x of up to 16 rows as two fp16 numbers: [block][register][lane group][row][hi, lo], [group][16] factors and [16]
-// sums.  A lane's sums are rows 4 (lane / 16) ..
+// sums, in the products' units.  A lane's sums are rows 4 (lane / 16) ..
 template <int GROUP_WORDS, bool LOWS>
 __global__ __launch_bounds__(kBlock) void connected4_halves_kernel(const float* x, char* parts, float* factors, uint32_t words,
                                                                    uint32_t blocks) {
@@ -288,10 +288,12 @@ __global__ __launch_bounds__(kBlock) void connected4_halves_kernel(const float* 
   }
   float most = 0.f, sum = 0.f;
 #pragma unroll
-  for (int c = 0; c < 8; ++c) most = larger(most, __builtin_fabsf(v[c])), sum += v[c];
+  for (int c = 0; c < 8; ++c) most = larger(most, __builtin_fabsf(v[c]));
   most = across_lanes<GROUP_WORDS>(most, [](float a, float b) { return larger(a, b); });
-  sum = across_lanes<GROUP_WORDS>(sum, [](float a, float b) { return a + b; });
   const int e = lift_of(most);
+#pragma unroll
+  for (int c = 0; c < 8; ++c) sum = __builtin_fmaf(v[c], power2(e), sum);
+  sum = across_lanes<GROUP_WORDS>(sum, [](float a, float b) { return a + b; });
   v8h hi, lo;
   operand_of(v, power2(e), hi, lo);
   int g, t;
@@ -323,26 +325,22 @@ struct HalfRows {
   }
   SHDW_DEVICE void multiply(const Operands& k, const float*, const float* factors, int g, const uint32_t (&w)[4],
                             const float (&step)[kGroups], const float (&low)[kGroups], float (&sums)[kSums]) const {
-    v4f part = {0.f, 0.f, 0.f, 0.f};
+    v4f part, sum;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const v8h b = operand_of(w[t]);
+      if (t % (GROUP_WORDS / 4) == 0) {
+        sum = *reinterpret_cast<const v4f*>(factors + t / (GROUP_WORDS / 4) * kFactors + 16 + 4 * g);
+        part = LOWS ? v4f{0.f, 0.f, 0.f, 0.f} : sum;
+      }
       part = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.hi[t], b, part, 0, 0, 0);
       part = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.lo[t], b, part, 0, 0, 0);
       if ((t + 1) % (GROUP_WORDS / 4) == 0) {
         const int u = t / (GROUP_WORDS / 4);
         const v4f undo = *reinterpret_cast<const v4f*>(factors + u * kFactors + 4 * g);
-        const v4f sum = *reinterpret_cast<const v4f*>(factors + u * kFactors + 16 + 4 * g);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (LOWS) {
-            sums[r] = __builtin_fmaf(part[r] * undo[r], step[u], sums[r]);
-            sums[r] = __builtin_fmaf(sum[r], low[u], sums[r]);
-          } else {
-            sums[r] = __builtin_fmaf(__builtin_fmaf(part[r], undo[r], sum[r]), step[u], sums[r]);
-          }
-        }
-        part = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < 4; ++r)
+          sums[r] = __builtin_fmaf(LOWS ? __builtin_fmaf(sum[r], low[u], part[r] * step[u]) : part[r] * step[u], undo[r], sums[r]);
       }
     }
   }
@@ -583,19 +581,19 @@ __global__ __launch_bounds__(kBlock) void connected4_split_kernel(const float* x
       const uint32_t w = (turn + n) * 32 + lane, stage = w / kStageWords;
       if (turn + n >= to) break;
       const bool real = there && w < words;
-      float v[8], sum = 0.f;
+      float v[8], group_most = 0.f, sum = 0.f;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         v[c] = real ? all[n][c] : 0.f;
-        sum += v[c];
+        group_most = larger(group_most, __builtin_fabsf(v[c]));
       }
-      float group_most = 0.f;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) group_most = larger(group_most, __builtin_fabsf(v[c]));
-      sum = across_lanes<GROUP_WORDS>(sum, [](float a, float b) { return a + b; });
       group_most = across_lanes<GROUP_WORDS>(group_most, [](float a, float b) { return larger(a, b); });
-      if (stage >= stages) continue;
       const int lift = group_most == 0.f || group_most >= most * kNear ? e : min(lift_of(group_most), e + kMostLift);
+      // in the units of the products, where they are added to them, else in the row's
+#pragma unroll
+      for (int c = 0; c < 8; ++c) sum = __builtin_fmaf(v[c], power2(LOWS ? e : lift), sum);
+      sum = across_lanes<GROUP_WORDS>(sum, [](float a, float b) { return a + b; });
+      if (stage >= stages) continue;
       own = own || lift != e;
       const int word = w % kStageWords;
       v8h hi, lo;
@@ -604,9 +602,8 @@ __global__ __launch_bounds__(kBlock) void connected4_split_kernel(const float* x
                  stage_lane(word, r);
       out[0] = hi;
       out[kStageBytes / 32] = lo;
-      // in the units of the products, where they are added to them, else in the row's
       float* const group = sums + (static_cast<uint64_t>(block) * stages + stage) * kStageSums + word / 4 * 32 + r;
-      if (w % GROUP_WORDS == 0) group[0] = LOWS ? sum * power2(e) : sum * power2(lift) * -8.f;
+      if (w % GROUP_WORDS == 0) group[0] = LOWS ? sum : sum * -8.f;
       if (w % min(GROUP_WORDS, kStageWords) == 0) group[64] = power2(e - lift);
     }
   }

@@ -45,3 +45,19 @@ def test_connected4_groups_of_very_different_sizes(gpu, rows, n_in, n_out, group
     bias = normal(86, n_out)
     y = run_connected4(x, codes, steps, low, bias, group)
     oracle.assert_within(y, *oracle.connected4(x, codes, steps, low, bias, group), "connected4")
+
+
+@pytest.mark.parametrize("rows,n_in,n_out,group", FORMS)
+@pytest.mark.parametrize("lows", [False, True])
+@pytest.mark.parametrize("size", [3e38, 2e35])
+def test_connected4_of_values_at_the_ends_of_the_range(gpu, rows, n_in, n_out, group, lows, size):
+    """Sums of code * x and of x may leave fp32's range where x and the result are within it."""
+    codes, steps, low = weights(87, n_in, n_out, group, lows)
+    steps *= F(1e-6)
+    if lows:
+        low *= F(1e-6)
+    x = (np.abs(normal(88, (rows, n_in))).clip(0, 1) * F(size)).astype(F)
+    y = run_connected4(x, codes, steps, low, None, group)
+    want, bound = oracle.connected4(x, codes, steps, low, None, group)
+    assert np.isfinite(y).all()
+    oracle.assert_within(y, want, bound, "connected4")
