@@ -128,14 +128,14 @@ SHDW_DEVICE Digits digits_of(const float (&v)[8]) {
 #pragma unroll
   for (int c = 0; c < 8; ++c) most = larger_or_nan(most, __builtin_fabsf(v[c]));
   most = across_lanes<GROUP_WORDS>(most, [](float a, float b) { return larger_or_nan(a, b); });
-  // the largest in [2^22, 2^23) / 1.0045: three digits hold up to 127 * 65793 = 2^23 / 1.0039
-  const int e = min(126, 22 - max(-104, exponent_of(most * 1.0045f)));
-  const float f = power2(e);
+  // the largest in [2^22, 2^23) / 1.0045: three digits hold up to 127 * 65793 = 2^23 / 1.0039; up to 2^148, in two steps
+  const int e = 22 - max(-126, exponent_of(most * 1.0045f));
+  const float f = power2(min(e, 126)), f2 = power2(max(e - 126, 0));
   uint32_t top[2] = {}, middle[2] = {}, low[2] = {};
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
     // v = 65536 a + 256 b + c, each in -128 .. 127
-    const float scaled = v[c] * f;
+    const float scaled = v[c] * f * f2;
     sum += scaled;
     const int d = static_cast<int>(__builtin_rintf(scaled));
     const int lo = static_cast<int8_t>(d), rest = (d - lo) >> 8, mid = static_cast<int8_t>(rest), hi = (rest - mid) >> 8;
@@ -146,7 +146,7 @@ SHDW_DEVICE Digits digits_of(const float (&v)[8]) {
   }
   Digits d;
   d.top = make_uint2(top[0], top[1]), d.middle = make_uint2(middle[0], middle[1]), d.low = make_uint2(low[0], low[1]);
-  d.factor = most < INFINITY ? power2(-e) : NAN;  // digits hold nothing that is not finite
+  d.factor = most < INFINITY ? __builtin_ldexpf(1.f, -e) : NAN;  // digits hold nothing that is not finite
   sum = across_lanes<GROUP_WORDS>(sum, [](float a, float b) { return a + b; });
   d.sum = LOWS ? sum : sum * -8.f;
   return d;
