@@ -18,8 +18,9 @@
 // contraction may take the keys in any order and the values are stored in that order.
 //
 // A tile is left to the fp32 instruction, from the caches themselves, where a power of two for the whole tile
-// would cost precision: where its rows differ in size by more than 2^12 or something in it is not
-// finite.  So a row that does not see (or hardly weighs) an outlier does not suffer from it.
+// would cost precision: where its keys differ in size by more than 2^12, where its values' rows and columns do (value_least), where
+// values in front of it were far smaller than its own (rough_values), or where something in it is not
+// finite.  So a row that does not see (or hardly weighs) an outlier, and a column that has none, does not suffer from it.
 //
 // A causal prompt of 4096 tokens, 32 heads of 128 values on 8: 391 us, 137 GFLOP of products or 1.06 PFLOP/s of fp16 ones, what
 // a large library product reaches; the split is 12 us of it.  577 patches that all see each other, 16 images, 12 heads of 64: 96 us,
@@ -41,8 +42,9 @@ constexpr int kWaveRows = 32;
 
 struct alignas(16) TileInfo {
   float key_factor;    // 2^-e of the keys
-  float value_factor;  // 2^-e of the values
-  int wild_keys, wild_values;
+  float value_factor;  // 2^-e of the values; NaN: they need fp32 operands
+  float value_least;   // the largest |value| of the row that has the smallest one, rows of zeros apart
+  int wild_keys;
 };
 
 // The tiles of 32 keys, counted from key 0, that queries between two reaches see: [0, sinks) and [lo, hi).
@@ -57,9 +59,11 @@ SHDW_DEVICE TileSpan span_of(const Reach& a, const Reach& b) {
   return s;
 }
 
-// The largest and the smallest row of a tile, from the largest |x| of each: powers of two and wildness.
+// The largest and the smallest row of a tile's keys, from the largest |x| of each.
 // Rows of zeros (and rows that nobody sees, which count as zeros) do not say how small a row is.
 SHDW_DEVICE bool is_wild(float largest, float smallest) { return !(largest < INFINITY) || largest > smallest * 4096.f; }
+
+constexpr int kMostLift = 30;  // of values, either way
 
 // A workgroup a tile, eight lanes a key, everything read once: keys stay in registers while the largest
 // values are found, values go through LDS, from where they are taken value by value.
@@ -67,7 +71,7 @@ template <int NB>
 __global__ __launch_bounds__(kBlock) void attention_split_kernel(const float* k, const float* v, v8h* parts, TileInfo* infos,
                                                                   FastDiv f_tiles, AttentionArgs p) {
   constexpr int kPadded = 32 * NB, kChunks = kPadded / 8, kEach = (kChunks + 7) / 8;  // chunks of 8 values, of a lane
-  __shared__ float most[2][kBlock / kWave], least[2][kBlock / kWave];
+  __shared__ float most[2][kBlock / kWave], least[2][kBlock / kWave], columns[2][kPadded];
   __shared__ v4f rows[kTile][kPadded / 4 + 1];  // keys start in other banks
   const int tid = threadIdx.x;
   uint32_t head, slot;
@@ -128,41 +132,40 @@ __global__ __launch_bounds__(kBlock) void attention_split_kernel(const float* k,
       rows[key][2 * (part + 8 * c) + 1] = v4f{x[1][c][4], x[1][c][5], x[1][c][6], x[1][c][7]};
     }
   __syncthreads();
-  float factor[2];
-  bool wild[2];
+  float largest[2], smallest[2];
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    float large = most[which][0], small = least[which][0];
+    largest[which] = most[which][0], smallest[which] = least[which][0];
 #pragma unroll
     for (int w = 1; w < kBlock / kWave; ++w) {
-      large = larger_or_nan(large, most[which][w]);
-      small = __builtin_fminf(small, least[which][w]);
-    }
-    wild[which] = is_wild(large, small);
-    if (which == 0) {
-      const int e = lift_of(large);
-      factor[0] = power2(e);
-      if (tid == 0) infos[blockIdx.x].key_factor = power2(-e);
-    } else {
-      // steps of 2^4, so that neighbouring tiles mostly agree: the largest in [2^10, 2^14)
-      const int e = large == 0.f ? 0 : 10 - (exponent_of(large) & ~3);
-      if (e > 30 || e < -30) wild[1] = true;  // sums in units of these could leave fp32's range
-      factor[1] = power2(wild[1] ? 0 : e);
-      if (tid == 0) infos[blockIdx.x].value_factor = power2(wild[1] ? 0 : -e);
+      largest[which] = larger_or_nan(largest[which], most[which][w]);
+      smallest[which] = __builtin_fminf(smallest[which], least[which][w]);
     }
   }
-  if (tid == 0) infos[blockIdx.x].wild_keys = wild[0], infos[blockIdx.x].wild_values = wild[1];
+  const bool wild_keys = is_wild(largest[0], smallest[0]);
+  const int key_lift = lift_of(largest[0]);
+  // Steps of 2^4, so that neighbouring tiles mostly agree: the largest in [2^10, 2^14).  In tiles that are not whole the
+  // smallest column may be a single small number: they have the most bits that there are.
+  const bool part_of_tile = !((tile + 1) * kTile <= last.first || (tile * kTile >= first.lo && (tile + 1) * kTile <= last.hi));
+  const int value_lift = largest[1] == 0.f ? kMostLift : part_of_tile ? 13 - exponent_of(largest[1]) : 10 - (exponent_of(largest[1]) & ~3);
+  // sums in units of these could leave fp32's range; 128 is what the exponent of infinities and NaN gives
+  const bool wild_values = value_lift > kMostLift || value_lift < -kMostLift;
+  if (tid == 0) {
+    infos[blockIdx.x].key_factor = power2(-key_lift), infos[blockIdx.x].wild_keys = wild_keys;
+    infos[blockIdx.x].value_least = smallest[1];
+    if (wild_values) infos[blockIdx.x].value_factor = NAN;
+  }
 
   // [keys hi][keys lo][values hi][values lo], each 32 * kPadded numbers
   constexpr uint32_t kQuarter = kTile * kPadded / 8;
   v8h* out = parts + static_cast<uint64_t>(blockIdx.x) * 4 * kQuarter;
-  if (!wild[0]) {
+  if (!wild_keys) {
 #pragma unroll
     for (int c = 0; c < kEach; ++c) {
       const int chunk = part + 8 * c;
       if (chunk >= kChunks) break;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[0][c][i] *= factor[0];
+      for (int i = 0; i < 8; ++i) x[0][c][i] *= power2(key_lift);
       v8h hi, lo;
       split8(x[0][c], hi, lo);
       const uint32_t at = (chunk / 2) * kWave + (chunk % 2) * 32 + key;
@@ -170,20 +173,40 @@ __global__ __launch_bounds__(kBlock) void attention_split_kernel(const float* k,
       out[kQuarter + at] = lo;
     }
   }
-  if (!wild[1]) {
-    const float* const values = reinterpret_cast<const float*>(rows);
+  if (wild_values) return;
+  const float* const values = reinterpret_cast<const float*>(rows);
 #pragma unroll
-    for (int n = tid; n < 4 * kPadded; n += kBlock) {
-      // value d of keys 16 m + 8 a + 4 h + t, element 4 a + t
-      const int d = n / 128 * 32 + n % 32, h = n / 32 % 2, m = n / 64 % 2;
-      float w[8];
+  for (int n = tid; n < 4 * kPadded; n += kBlock) {
+    // value d of keys 16 m + 8 a + 4 h + t, element 4 a + t
+    const int d = n / 128 * 32 + n % 32, h = n / 32 % 2, m = n / 64 % 2;
+    float w[8], column = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = values[(16 * m + 8 * (i / 4) + 4 * h + i % 4) * (kPadded + 4) + d] * factor[1];
-      v8h hi, lo;
-      split8(w, hi, lo);
-      out[2 * kQuarter + n] = hi;
-      out[3 * kQuarter + n] = lo;
+    for (int i = 0; i < 8; ++i) {
+      w[i] = values[(16 * m + 8 * (i / 4) + 4 * h + i % 4) * (kPadded + 4) + d];
+      column = larger(column, __builtin_fabsf(w[i]));
+      w[i] *= power2(value_lift);
     }
+    column = across_halves(column, larger);  // of keys 16 m ..
+    if (h == 0) columns[m][d] = column;
+    v8h hi, lo;
+    split8(w, hi, lo);
+    out[2 * kQuarter + n] = hi;
+    out[3 * kQuarter + n] = lo;
+  }
+  // Where rows and columns differ in size, values of a small row in a small column are about (smallest row) (smallest column) /
+  // largest.  What the second part of a number rounds away is up to 2^-25 in units of the lift; it has to be less
+  // than 2^-21 of those.
+  __syncthreads();
+  if (tid >= kWave) return;
+  float column = INFINITY;
+  for (int d = tid; d < kPadded; d += kWave) {
+    const float c = larger(columns[0][d], columns[1][d]);
+    if (c > 0.f) column = __builtin_fminf(column, c);
+  }
+  for (int step = 1; step < kWave; step <<= 1) column = __builtin_fminf(column, __shfl_xor(column, step));
+  if (tid == 0) {
+    const float factor = power2(-value_lift), small = smallest[1] / largest[1] * column;
+    infos[blockIdx.x].value_factor = largest[1] == 0.f || factor <= 16.f * small ? factor : NAN;
   }
 }
 
@@ -198,9 +221,11 @@ SHDW_DEVICE void fetch(const char* from, char* to, int wave, int lane) {
   }
 }
 
-// The weights that go to the second product are 2^(score - top + 10): at most 2^15 while `top` lags behind
-// by up to kLag, and down to 2^-34 of the largest before fp16 rounds them away.
-constexpr float kLift = 10.f, kLag = 5.f;
+// The weights that go to the second product are 2^(score - top + 12): at most 2^15 while `top` lags behind
+// by up to kLag, and down to 2^-37 of the largest before fp16 rounds them away.  What is rounded away counts as its values do:
+// a tile whose values are up to 2^12 times the smallest row's in front of it adds 2^-25 of these for a key at most, others have fp32
+// weights.
+constexpr float kLift = 12.f, kLag = 3.f;
 
 // The tiles that go through fp32 operands are rare and their code is long: functions of their own, so that the
 // others' registers do not depend on them.
@@ -343,7 +368,7 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
     const InfoPointer at = tile_infos + slot_at(tile_at(n));
     TileInfo info;
     info.key_factor = at->key_factor, info.value_factor = at->value_factor;
-    info.wild_keys = at->wild_keys, info.wild_values = at->wild_values;
+    info.value_least = at->value_least, info.wild_keys = at->wild_keys;
     return info;
   };
   const auto ask = [&](int n, int buffer) {
@@ -354,6 +379,8 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
     for (int a = 0; a < kAhead; ++a) ask(from + a, a);
   }
   int buffer = 0;
+  // the least row of the tiles so far; positive numbers compare like their bits, and these can stay in scalar registers
+  uint32_t least = __float_as_uint(INFINITY);
   for (int n = from; n < to; ++n) {
     const int tile = tile_at(n), j0 = tile * kTile;
     const char* here = lds[buffer];
@@ -420,7 +447,10 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
     }
     total += part_sum;
 
-    if (!info.wild_values) {
+    least = min(least, __float_as_uint(info.value_least));
+    // 4 value_factor > least, where the largest is less than 2^14 times value_factor; or a NaN
+    const bool rough_values = __float_as_uint(info.value_factor) + (2u << 23) > least;
+    if (!rough_values) {
       if (info.value_factor != unit) {
         const float g = unit * (1.f / info.value_factor);  // powers of two
         unit = info.value_factor;

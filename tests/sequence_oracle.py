@@ -114,3 +114,36 @@ def assert_within(got, want, bound, what=""):
         at = np.unravel_index(np.argmax(np.where(bad, off / np.maximum(bound, 1e-300), 0)), off.shape)
         raise AssertionError("%s: %d of %d outside; worst at %s: got %r want %r, off %.3g, allowed %.3g" % (
             what, bad.sum(), off.size, at, got[at], want[at], off[at], bound[at]))
+
+
+def attention_of_head(q, k, v, start, keys, window, sinks, causal, scale):
+    """(y, bound) of one head of one sequence: q [n][dim] from position `start` on, k and v [at least keys][dim].
+
+    The bound of a value is relative to its own column, and to what the weights leave of it: sum_j w_j |v_j| times the
+    same roundings as in window_attention.  So it does not grow with columns, keys or values that the result does not depend on."""
+    q, k, v = np.asarray(q, np.float64), np.asarray(k, np.float64)[:keys], np.asarray(v, np.float64)[:keys]
+    n, dim = q.shape
+    seen = np.zeros((n, keys), bool)
+    for t in range(n):
+        seen[t] = reach(start + t, keys, window, sinks, causal)
+    if not seen.any():
+        return np.zeros_like(q), np.zeros_like(q)
+    s = scale * (q @ k.T)
+    off = abs(scale) * (np.abs(q) @ np.abs(k).T) * (2.0 ** -21 + dim * HALF) + np.abs(s) * 3 * HALF
+    d = np.where(seen, off, 0.0).max(1, keepdims=True)
+    top = np.where(seen, s, -np.inf).max(1, keepdims=True)
+    w = np.where(seen, np.exp(np.minimum(s - np.where(np.isfinite(top), top, 0.0), 0.0)), 0.0)
+    w /= np.maximum(w.sum(1, keepdims=True), 1e-300)
+    count = seen.sum(1, keepdims=True)
+    return w @ v, (w @ np.abs(v)) * (2 * d + 2.0 ** -20 + (32 + count / 16) * HALF) + 1e-37
+
+
+def attention_by_heads(y, q, k, v, starts, lengths, window, sinks, causal, scale, pairs=None, what="attention"):
+    """Holds y against attention_of_head, for all (sequence, query head) or the `pairs` given."""
+    batch, length, q_heads, _ = q.shape
+    group, capacity = q_heads // k.shape[1], k.shape[2]
+    for b, h in pairs or [(b, h) for b in range(batch) for h in range(q_heads)]:
+        n = min(max(int(lengths[b]), 0), length)
+        keys = min(max(int(starts[b]) + n, 0), capacity)
+        want, bound = attention_of_head(q[b, :n, h], k[b, h // group], v[b, h // group], int(starts[b]), keys, window, sinks, causal, scale)
+        assert_within(y[b, :n, h], want, bound, "%s, head %d of sequence %d" % (what, h, b))

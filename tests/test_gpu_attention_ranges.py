@@ -5,10 +5,16 @@ import pytest
 
 from tests import sequence_oracle as oracle
 from tests.helpers import normal, rng
-from tests.test_gpu_attention_layer import run_connected4, weights
+from tests.test_gpu_attention_layer import inputs, run_attention, run_connected4, weights
 
 pytestmark = pytest.mark.gpu
 F = np.float32
+
+
+def away(seed, shape):
+    """Numbers of either sign, from 0.5 to 1.5 in size."""
+    g = rng(seed)
+    return ((0.5 + g.random(shape)) * np.where(g.random(shape) < 0.5, -1, 1)).astype(F)
 
 
 # rows, in, out, group: one row, two to eight, by sixteen, and in tiles (more than 4096 rows)
@@ -63,3 +69,38 @@ def test_connected4_of_values_at_the_ends_of_the_range(gpu, rows, n_in, n_out, g
     assert np.isfinite(y).all()
     # results of 1e-37 are near the least normal number: what is subnormal on the way has steps of 2^-149
     oracle.assert_within(y, want, bound - 1e-37 + n_in * 2.0 ** -148, "connected4")
+
+
+# batch, length, q_heads, kv_heads: a token, a few rows, tiles
+SPANS = [(2, 1, 4, 2), (1, 3, 4, 2), (1, 70, 4, 2), (1, 200, 2, 2)]
+
+
+@pytest.mark.parametrize("batch,length,q_heads,kv_heads", SPANS)
+@pytest.mark.parametrize("dim", [64, 100, 128, 160])
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e9, 1e15])
+def test_attention_of_a_column_far_larger_than_the_others(gpu, batch, length, q_heads, kv_heads, dim, size):
+    """One column of v is `size` times the others: they do not depend on it."""
+    capacity = 300
+    q, k, _ = inputs(91, batch, length, q_heads, kv_heads, dim, capacity)
+    v = away(92, (batch, kv_heads, capacity, dim))
+    v[..., 17] *= F(size)
+    args = ([capacity - length] * batch, [length] * batch, 0, 0, 1, dim ** -0.5)
+    oracle.attention_by_heads(run_attention(q, k, v, *args), q, k, v, *args)
+
+
+@pytest.mark.parametrize("batch,length,q_heads,kv_heads", SPANS)
+@pytest.mark.parametrize("size", [30, 1e4, 1e7, 1e9, 1e12])
+@pytest.mark.parametrize("period", [1, 32, 90])
+def test_attention_of_large_values_with_small_weights(gpu, batch, length, q_heads, kv_heads, size, period):
+    """Every other `period` keys have values `size` times the others' and weights smaller by as much or more."""
+    capacity, dim = 400, 64
+    q, k, _ = inputs(95, batch, length, q_heads, kv_heads, dim, capacity)
+    v = away(96, (batch, kv_heads, capacity, dim))
+    large = np.arange(capacity) // period % 2 == 1
+    v[:, :, large] *= F(size)
+    q[..., 0], k[..., 0] = 4, 0
+    k[:, :, large, 0] = F(-np.log(size) / (4 * 0.125))
+    for extra in (0, 4):
+        k[:, :, large, 0] -= F(extra)
+        args = ([capacity - length] * batch, [length] * batch, 0, 0, 1, 0.125)
+        oracle.attention_by_heads(run_attention(q, k, v, *args), q, k, v, *args)
