@@ -17,9 +17,9 @@
 // lane, rounded to hi and lo, are the operand of the second product as they are, since its
 // contraction may take the keys in any order and the values are stored in that order.
 //
-// A tile is left to the fp32 instruction, from the caches themselves, where a power of two for the whole tile
-// would cost precision: where its keys differ in size by more than 2^12, where its values' rows and columns do (value_least), where
-// values in front of it were far smaller than its own (rough_values), or where something in it is not
+// A tile is left to the fp32 instruction, from the caches themselves, where a power of two for the whole tile or row
+// would cost precision: where that shows in the scores (rough_keys), where its values' rows and columns differ in size (value_factor),
+// where values in front of it were far smaller than its own (rough_values), or where something in it is not
 // finite.  So a row that does not see (or hardly weighs) an outlier, and a column that has none, does not suffer from it.
 //
 // A causal prompt of 4096 tokens, 32 heads of 128 values on 8: 391 us, 137 GFLOP of products or 1.06 PFLOP/s of fp16 ones, what
@@ -33,6 +33,8 @@
 #include "launch.h"
 #include "split16.h"
 
+#include <type_traits>
+
 #pragma clang fp contract(off)
 
 namespace shdw {
@@ -42,9 +44,9 @@ constexpr int kWaveRows = 32;
 
 struct alignas(16) TileInfo {
   float key_factor;    // 2^-e of the keys
+  float key_sum;       // the largest sum of |x| of a key
   float value_factor;  // 2^-e of the values; NaN: they need fp32 operands
   float value_least;   // the largest |value| of the row that has the smallest one, rows of zeros apart
-  int wild_keys;
 };
 
 // The tiles of 32 keys, counted from key 0, that queries between two reaches see: [0, sinks) and [lo, hi).
@@ -59,10 +61,6 @@ SHDW_DEVICE TileSpan span_of(const Reach& a, const Reach& b) {
   return s;
 }
 
-// The largest and the smallest row of a tile's keys, from the largest |x| of each.
-// Rows of zeros (and rows that nobody sees, which count as zeros) do not say how small a row is.
-SHDW_DEVICE bool is_wild(float largest, float smallest) { return !(largest < INFINITY) || largest > smallest * 4096.f; }
-
 constexpr int kMostLift = 30;  // of values, either way
 
 // A workgroup a tile, eight lanes a key, everything read once: keys stay in registers while the largest
@@ -71,7 +69,7 @@ template <int NB>
 __global__ __launch_bounds__(kBlock) void attention_split_kernel(const float* k, const float* v, v8h* parts, TileInfo* infos,
                                                                   FastDiv f_tiles, AttentionArgs p) {
   constexpr int kPadded = 32 * NB, kChunks = kPadded / 8, kEach = (kChunks + 7) / 8;  // chunks of 8 values, of a lane
-  __shared__ float most[2][kBlock / kWave], least[2][kBlock / kWave], columns[2][kPadded];
+  __shared__ float most[2][kBlock / kWave], other[2][kBlock / kWave], columns[2][kPadded];  // other: sums of keys, the least values
   __shared__ v4f rows[kTile][kPadded / 4 + 1];  // keys start in other banks
   const int tid = threadIdx.x;
   uint32_t head, slot;
@@ -110,20 +108,30 @@ __global__ __launch_bounds__(kBlock) void attention_split_kernel(const float* k,
     }
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    float m = 0.f;
+    float m = 0.f, sum = 0.f;
 #pragma unroll
     for (int c = 0; c < kEach; ++c)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = larger_or_nan(m, __builtin_fabsf(x[which][c][i]));
+      for (int i = 0; i < 8; ++i) {
+        m = larger_or_nan(m, __builtin_fabsf(x[which][c][i]));
+        if (which == 0) sum += __builtin_fabsf(x[which][c][i]);
+      }
     m = larger_or_nan(m, dpp_f32<kDppXor1>(m));
     m = larger_or_nan(m, dpp_f32<kDppXor2>(m));
     m = larger_or_nan(m, dpp_f32<kDppHalfMirror>(m));
-    float large = m, small = m == 0.f ? INFINITY : m;
-    for (int step = 8; step < kWave; step <<= 1) {
-      large = larger_or_nan(large, __shfl_xor(large, step));
-      small = __builtin_fminf(small, __shfl_xor(small, step));
+    if (which == 0) {
+      sum += dpp_f32<kDppXor1>(sum);
+      sum += dpp_f32<kDppXor2>(sum);
+      sum += dpp_f32<kDppHalfMirror>(sum);
+    } else {
+      sum = m == 0.f ? -INFINITY : -m;
     }
-    if (tid % kWave == 0) most[which][tid / kWave] = large, least[which][tid / kWave] = small;
+    for (int step = 8; step < kWave; step <<= 1) {
+      m = larger_or_nan(m, __shfl_xor(m, step));
+      const float next = __shfl_xor(sum, step);
+      sum = which == 0 ? larger_or_nan(sum, next) : larger(sum, next);
+    }
+    if (tid % kWave == 0) most[which][tid / kWave] = m, other[which][tid / kWave] = sum;
   }
 #pragma unroll
   for (int c = 0; c < kEach; ++c)
@@ -132,17 +140,13 @@ __global__ __launch_bounds__(kBlock) void attention_split_kernel(const float* k,
       rows[key][2 * (part + 8 * c) + 1] = v4f{x[1][c][4], x[1][c][5], x[1][c][6], x[1][c][7]};
     }
   __syncthreads();
-  float largest[2], smallest[2];
+  float largest[2] = {most[0][0], most[1][0]}, key_sum = other[0][0], smallest = -other[1][0];
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    largest[which] = most[which][0], smallest[which] = least[which][0];
-#pragma unroll
-    for (int w = 1; w < kBlock / kWave; ++w) {
-      largest[which] = larger_or_nan(largest[which], most[which][w]);
-      smallest[which] = __builtin_fminf(smallest[which], least[which][w]);
-    }
+  for (int w = 1; w < kBlock / kWave; ++w) {
+    largest[0] = larger_or_nan(largest[0], most[0][w]), largest[1] = larger_or_nan(largest[1], most[1][w]);
+    key_sum = larger_or_nan(key_sum, other[0][w]);
+    smallest = __builtin_fminf(smallest, -other[1][w]);
   }
-  const bool wild_keys = is_wild(largest[0], smallest[0]);
   const int key_lift = lift_of(largest[0]);
   // Steps of 2^4, so that neighbouring tiles mostly agree: the largest in [2^10, 2^14).  In tiles that are not whole the
   // smallest column may be a single small number: they have the most bits that there are.
@@ -151,27 +155,25 @@ __global__ __launch_bounds__(kBlock) void attention_split_kernel(const float* k,
   // sums in units of these could leave fp32's range; 128 is what the exponent of infinities and NaN gives
   const bool wild_values = value_lift > kMostLift || value_lift < -kMostLift;
   if (tid == 0) {
-    infos[blockIdx.x].key_factor = power2(-key_lift), infos[blockIdx.x].wild_keys = wild_keys;
-    infos[blockIdx.x].value_least = smallest[1];
+    infos[blockIdx.x].key_factor = power2(-key_lift), infos[blockIdx.x].key_sum = key_sum;
+    infos[blockIdx.x].value_least = smallest;
     if (wild_values) infos[blockIdx.x].value_factor = NAN;
   }
 
   // [keys hi][keys lo][values hi][values lo], each 32 * kPadded numbers
   constexpr uint32_t kQuarter = kTile * kPadded / 8;
   v8h* out = parts + static_cast<uint64_t>(blockIdx.x) * 4 * kQuarter;
-  if (!wild_keys) {
 #pragma unroll
-    for (int c = 0; c < kEach; ++c) {
-      const int chunk = part + 8 * c;
-      if (chunk >= kChunks) break;
+  for (int c = 0; c < kEach; ++c) {
+    const int chunk = part + 8 * c;
+    if (chunk >= kChunks) break;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[0][c][i] *= power2(key_lift);
-      v8h hi, lo;
-      split8(x[0][c], hi, lo);
-      const uint32_t at = (chunk / 2) * kWave + (chunk % 2) * 32 + key;
-      out[at] = hi;
-      out[kQuarter + at] = lo;
-    }
+    for (int i = 0; i < 8; ++i) x[0][c][i] *= power2(key_lift);
+    v8h hi, lo;
+    split8(x[0][c], hi, lo);
+    const uint32_t at = (chunk / 2) * kWave + (chunk % 2) * 32 + key;
+    out[at] = hi;
+    out[kQuarter + at] = lo;
   }
   if (wild_values) return;
   const float* const values = reinterpret_cast<const float*>(rows);
@@ -205,7 +207,7 @@ __global__ __launch_bounds__(kBlock) void attention_split_kernel(const float* k,
   }
   for (int step = 1; step < kWave; step <<= 1) column = __builtin_fminf(column, __shfl_xor(column, step));
   if (tid == 0) {
-    const float factor = power2(-value_lift), small = smallest[1] / largest[1] * column;
+    const float factor = power2(-value_lift), small = smallest / largest[1] * column;
     infos[blockIdx.x].value_factor = largest[1] == 0.f || factor <= 16.f * small ? factor : NAN;
   }
 }
@@ -229,49 +231,41 @@ constexpr float kLift = 12.f, kLag = 3.f;
 
 // The tiles that go through fp32 operands are rare and their code is long: functions of their own, so that the
 // others' registers do not depend on them.
-// Scores of a tile with the rows' operands q [2 NB][hi, lo].
+// Scores of a tile, a lane's key and row given, as the kernel for few rows has them.
 template <int NB>
-__device__ __attribute__((noinline)) void wild_scores(const float* row, int dim, const v8h* q, float* scores) {
+__device__ __attribute__((noinline)) v16f fp32_scores(const float* key, const float* row, int dim, float scale) {
   const int half = threadIdx.x % kWave / 32;
   v16f s = {};
 #pragma unroll 1
   for (int c = 0; c < 2 * NB; ++c) {
-    const v8h hi = q[2 * c], lo = q[2 * c + 1];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int d = 16 * c + 8 * half + e;
-      s = __builtin_amdgcn_mfma_f32_32x32x2f32(d < dim ? row[d] : 0.f, static_cast<float>(hi[e]) + static_cast<float>(lo[e]), s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(d < dim ? key[d] : 0.f, d < dim ? row[d] * scale : 0.f, s, 0, 0, 0);
     }
   }
-#pragma unroll
-  for (int r = 0; r < 16; ++r) scores[r] = s[r];
+  return s;
 }
-// Adds the values of the tile from key j0 on, weighted, to acc [NB][16].  Whether a row sees a value that is not
-// finite; such values count as zeros.
-template <int NB>
-__device__ __attribute__((noinline)) bool wild_values(const float* values, int dim, int j0, int keys, Reach reach, const float* weights,
-                                                      float* acc) {
+// `sum` and up to 32 dims of the tile's values from key j0 on, weighted.  Values that are not finite count as zeros; a row that
+// sees one becomes NaN.
+__device__ __attribute__((noinline)) v16f fp32_values(const float* values, int dim, int dims, int j0, int keys, Reach reach, v16f weights,
+                                                      v16f sum) {
   const int lane = threadIdx.x % kWave, half = lane / 32, i = lane % 32;
   bool hurt = false;
-#pragma unroll 1
-  for (int b = 0; b < NB; ++b) {
-    v16f sum;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sum[r] = acc[16 * b + r];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int j = j0 + 8 * (r / 4) + 4 * half + r % 4;
-      float x = j < keys && 32 * b + i < dim ? values[static_cast<uint64_t>(j) * dim + 32 * b + i] : 0.f;
-      const bool off = !(__builtin_fabsf(x) < INFINITY);
-      x = off ? 0.f : x;
-      sum = __builtin_amdgcn_mfma_f32_32x32x2f32(x, weights[r], sum, 0, 0, 0);
-      const uint64_t votes = __builtin_amdgcn_ballot_w64(off);
-      hurt = hurt || (static_cast<uint32_t>(votes >> (32 * half)) != 0 && sees(reach, j));
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[16 * b + r] = sum[r];
+  for (int r = 0; r < 16; ++r) {
+    const int j = j0 + 8 * (r / 4) + 4 * half + r % 4;
+    float x = j < keys && i < dims ? values[static_cast<uint64_t>(j) * dim + i] : 0.f;
+    const bool off = !(__builtin_fabsf(x) < INFINITY);
+    x = off ? 0.f : x;
+    sum = __builtin_amdgcn_mfma_f32_32x32x2f32(x, weights[r], sum, 0, 0, 0);
+    const uint64_t votes = __builtin_amdgcn_ballot_w64(off);
+    hurt = hurt || (static_cast<uint32_t>(votes >> (32 * half)) != 0 && sees(reach, j));
   }
-  return hurt;
+  const float bad = across_halves(hurt ? 1.f : 0.f, larger) != 0.f ? NAN : 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) sum[r] += bad;
+  return sum;
 }
 
 // A wave has 32 rows.  Tiles are copied to LDS up to BUFFERS - 1 ahead of their use.
@@ -327,18 +321,59 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
   const uint64_t cache = static_cast<uint64_t>(head) * p.capacity * p.dim;
   const char* tile_parts = reinterpret_cast<const char*>(parts) + static_cast<uint64_t>(head) * tiles * kBytes;
 
+  const int count = span.sinks + span.hi - span.lo;
+  int from, to;
+  part_of(count, part, f_splits, from, to);
+  const auto tile_at = [&](int n) { return n < span.sinks ? n : span.lo + n - span.sinks; };
+  const auto slot_at = [&](int tile) { return tile < whole.sinks ? tile : tile - whole.lo + whole.sinks; };
+  // A tile's info comes by scalar loads, which are counted apart from the copies that are under way.
+  typedef const __attribute__((address_space(4))) TileInfo* InfoPointer;
+  const InfoPointer tile_infos = reinterpret_cast<InfoPointer>(reinterpret_cast<uintptr_t>(infos + static_cast<uint64_t>(head) * tiles));
+  const auto info_at = [&](int n) {
+    const InfoPointer at = tile_infos + slot_at(tile_at(n));
+    TileInfo info;
+    info.key_factor = at->key_factor, info.value_factor = at->value_factor;
+    info.value_least = at->value_least, info.key_sum = at->key_sum;
+    return info;
+  };
+  // What all tiles of the part have in common, a lane a tile: asked for here, in front of the copies.
+  uint32_t most_factor = 0, least_value = __float_as_uint(INFINITY);  // positive numbers compare like their bits
+  float key_sum = 0.f, key_factor = 0.f;
+  for (int n = from + lane; n < to; n += kWave) {
+    const TileInfo info = infos[static_cast<uint64_t>(head) * tiles + slot_at(tile_at(n))];
+    key_sum = larger_or_nan(key_sum, info.key_sum), key_factor = larger(key_factor, info.key_factor);
+    most_factor = max(most_factor, __float_as_uint(info.value_factor));
+    least_value = min(least_value, __float_as_uint(info.value_least));
+  }
+  const auto ask = [&](int n, int buffer) {
+    if (n < to) fetch<kBytes, WAVES>(tile_parts + static_cast<uint64_t>(slot_at(tile_at(n))) * kBytes, lds[buffer], wave, lane);
+  };
+  if (from < to) {
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) ask(from + a, a);
+  }
+
   v8h qhi[2 * NB], qlo[2 * NB];
-  float row_factor;
+  float row_factor, wave_most, wave_sum;  // of the wave's rows
   {
-    float m = 0.f;
+    float m = 0.f, sum = 0.f;
 #pragma unroll
     for (int s = 0; s < 2 * NB; ++s)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         x[s][e] = 16 * s + 8 * half + e < p.dim ? x[s][e] * (p.scale * kLog2e) : 0.f;
         m = larger(m, __builtin_fabsf(x[s][e]));
+        sum += __builtin_fabsf(x[s][e]);
       }
-    const int e = lift_of(across_halves(m, larger));
+    m = across_halves(m, larger);
+    wave_most = mine ? m : 0.f, wave_sum = mine ? across_halves(sum, plus) : 0.f;
+    for (int step = 1; step < 32; step <<= 1) {
+      wave_most = larger(wave_most, __shfl_xor(wave_most, step));
+      wave_sum = larger(wave_sum, __shfl_xor(wave_sum, step));
+    }
+    wave_most = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(wave_most)));
+    wave_sum = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(wave_sum)));
+    const int e = lift_of(m);
     const float f = power2(e);
     row_factor = power2(-e);
 #pragma unroll
@@ -356,144 +391,125 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
     for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
   float top = -INFINITY, total = 0.f, unit = 1.f;  // acc is in units of `unit`, a tile's value_factor
 
-  const int count = span.sinks + span.hi - span.lo;
-  int from, to;
-  part_of(count, part, f_splits, from, to);
-  const auto tile_at = [&](int n) { return n < span.sinks ? n : span.lo + n - span.sinks; };
-  const auto slot_at = [&](int tile) { return tile < whole.sinks ? tile : tile - whole.lo + whole.sinks; };
-  // A tile's info comes by scalar loads, which are counted apart from the copies that are under way.
-  typedef const __attribute__((address_space(4))) TileInfo* InfoPointer;
-  const InfoPointer tile_infos = reinterpret_cast<InfoPointer>(reinterpret_cast<uintptr_t>(infos + static_cast<uint64_t>(head) * tiles));
-  const auto info_at = [&](int n) {
-    const InfoPointer at = tile_infos + slot_at(tile_at(n));
-    TileInfo info;
-    info.key_factor = at->key_factor, info.value_factor = at->value_factor;
-    info.value_least = at->value_least, info.wild_keys = at->wild_keys;
-    return info;
-  };
-  const auto ask = [&](int n, int buffer) {
-    if (n < to) fetch<kBytes, WAVES>(tile_parts + static_cast<uint64_t>(slot_at(tile_at(n))) * kBytes, lds[buffer], wave, lane);
-  };
-  if (from < to) {
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) ask(from + a, a);
-  }
+  // What the second parts of keys and rows round away, up to 2^-38 of a row's and of a tile's largest number, adds up to 2^-38 of
+  // this in a score; it stays below 2^-22, whatever the scores (in powers of two) are.  Scores of thousands go through fp32, and so
+  // does a tile that holds something that is not finite.
+  const auto rough_scores = [&](float sum, float factor) { return !(wave_most * sum + wave_sum * (factor * 0x1p14f) <= 0x1p16f); };
+  // Values of a tile, less than 2^14 times their factor, are up to 2^12 times the least row's, or need fp32 weights; so does a
+  // factor that is a NaN.
+  const auto rough_weights = [](uint32_t factor, uint32_t least) { return factor + (2u << 23) > least; };
+  for (int step = 1; step < kWave; step <<= 1) least_value = min(least_value, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least_value), step)));
+  // Mostly nothing is rough: a loop that does not ask (for NB of 8 the other one has no room for its registers).
+  const bool smooth = __builtin_amdgcn_ballot_w64(rough_scores(key_sum, key_factor) || rough_weights(most_factor, least_value)) == 0;
   int buffer = 0;
-  // the least row of the tiles so far; positive numbers compare like their bits, and these can stay in scalar registers
-  uint32_t least = __float_as_uint(INFINITY);
-  for (int n = from; n < to; ++n) {
-    const int tile = tile_at(n), j0 = tile * kTile;
-    const char* here = lds[buffer];
-    const TileInfo info = info_at(n);  // in front of the wait: reads of LDS behind it are then counted alone
-    // the tile is there (later ones may be under way), and nobody reads the buffer that is filled next
-    if (to - n >= kAhead) copies_done<(kAhead - 1) * kBytes / (WAVES * kWave * 16)>();
-    else copies_done<0>();
-    ask(n + kAhead, buffer == 0 ? BUFFERS - 1 : buffer - 1);
-    buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
-    // a tile that none of the wave's rows sees
-    if (!(j0 < wave_b.first || (j0 < wave_b.hi && j0 + kTile > wave_a.lo))) continue;
+  uint32_t least = __float_as_uint(INFINITY);  // of the tiles so far, in a scalar register
+  const auto all = [&](auto ask_each) {
+    constexpr bool kAsk = decltype(ask_each)::value;
+    for (int n = from; n < to; ++n) {
+      const int tile = tile_at(n), j0 = tile * kTile;
+      const char* here = lds[buffer];
+      const TileInfo info = info_at(n);  // in front of the wait: reads of LDS behind it are then counted alone
+      // the tile is there (later ones may be under way), and nobody reads the buffer that is filled next
+      if (to - n >= kAhead) copies_done<(kAhead - 1) * kBytes / (WAVES * kWave * 16)>();
+      else copies_done<0>();
+      ask(n + kAhead, buffer == 0 ? BUFFERS - 1 : buffer - 1);
+      buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
+      // a tile that none of the wave's rows sees
+      if (!(j0 < wave_b.first || (j0 < wave_b.hi && j0 + kTile > wave_a.lo))) continue;
 
-    v16f s;
+      v16f s;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.f;
-    float f;
-    if (!info.wild_keys) {
-      const v8h* frag = reinterpret_cast<const v8h*>(here) + lane;
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
+      float f;
+      const bool rough_keys = kAsk && rough_scores(info.key_sum, info.key_factor);
+      if (!rough_keys) {
+        const v8h* frag = reinterpret_cast<const v8h*>(here) + lane;
 #pragma unroll
-      for (int c = 0; c < 2 * NB; ++c) {
-        const v8h hi = frag[c * kWave], lo = frag[(2 * NB + c) * kWave];
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qhi[c], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qlo[c], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, qhi[c], s, 0, 0, 0);
+        for (int c = 0; c < 2 * NB; ++c) {
+          const v8h hi = frag[c * kWave], lo = frag[(2 * NB + c) * kWave];
+          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qhi[c], s, 0, 0, 0);
+          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qlo[c], s, 0, 0, 0);
+          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, qhi[c], s, 0, 0, 0);
+        }
+        f = __builtin_fmaxf(__builtin_fminf(row_factor * info.key_factor, 0x1p127f), 0x1p-126f);  // neither 0 nor infinite
+      } else {
+        s = fp32_scores<NB>(k + cache + static_cast<uint64_t>(min(j0 + i, p.capacity - 1)) * p.dim, q + at, p.dim, p.scale * kLog2e);
+        f = 1.f;
+        loads_done();
       }
-      f = __builtin_fmaxf(__builtin_fminf(row_factor * info.key_factor, 0x1p127f), 0x1p-126f);  // neither 0 nor infinite
-    } else {
-      v8h operands[4 * NB];
-      float scores[16];
+      if (!((j0 + kTile <= wave_a.first) || (j0 >= wave_b.lo && j0 + kTile <= wave_a.hi))) {
 #pragma unroll
-      for (int c = 0; c < 2 * NB; ++c) operands[2 * c] = qhi[c], operands[2 * c + 1] = qlo[c];
-      wild_scores<NB>(k + cache + static_cast<uint64_t>(min(j0 + i, p.capacity - 1)) * p.dim, p.dim, operands, scores);
+        for (int r = 0; r < 16; ++r)
+          if (!sees(reach, j0 + 8 * (r / 4) + 4 * half + r % 4)) s[r] = -INFINITY;
+      }
+      float m = s[0];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = scores[r];
-      f = row_factor;
-      loads_done();
-    }
-    if (!((j0 + kTile <= wave_a.first) || (j0 >= wave_b.lo && j0 + kTile <= wave_a.hi))) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (!sees(reach, j0 + 8 * (r / 4) + 4 * half + r % 4)) s[r] = -INFINITY;
-    }
-    float m = s[0];
-#pragma unroll
-    for (int r = 1; r < 16; ++r) m = larger(m, s[r]);
-    m = across_halves(m, larger);
-    m = m == -INFINITY ? m : m * f;
-    if (__builtin_amdgcn_ballot_w64(m > top + kLag) != 0) {
-      const float next = larger(m, top);
-      const float g = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
-      top = next;
-      total *= g;
-#pragma unroll
-      for (int b2 = 0; b2 < NB; ++b2)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[b2][r] *= g;
-    }
-    const float shift = (top == -INFINITY ? 0.f : top) - kLift;
-    float part_sum = 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], f, -shift));
-      part_sum += s[r];
-    }
-    total += part_sum;
-
-    least = min(least, __float_as_uint(info.value_least));
-    // 4 value_factor > least, where the largest is less than 2^14 times value_factor; or a NaN
-    const bool rough_values = __float_as_uint(info.value_factor) + (2u << 23) > least;
-    if (!rough_values) {
-      if (info.value_factor != unit) {
-        const float g = unit * (1.f / info.value_factor);  // powers of two
-        unit = info.value_factor;
+      for (int r = 1; r < 16; ++r) m = larger(m, s[r]);
+      m = across_halves(m, larger);
+      m = m == -INFINITY ? m : m * f;
+      if (__builtin_amdgcn_ballot_w64(m > top + kLag) != 0) {
+        const float next = larger(m, top);
+        const float g = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
+        top = next;
+        total *= g;
 #pragma unroll
         for (int b2 = 0; b2 < NB; ++b2)
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[b2][r] *= g;
       }
-      v8h whi[2], wlo[2];
+      const float shift = (top == -INFINITY ? 0.f : top) - kLift;
+      float part_sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float w[8] = {s[8 * c], s[8 * c + 1], s[8 * c + 2], s[8 * c + 3], s[8 * c + 4], s[8 * c + 5], s[8 * c + 6], s[8 * c + 7]};
-        split8(w, whi[c], wlo[c]);
+      for (int r = 0; r < 16; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], f, -shift));
+        part_sum += s[r];
       }
-      const v8h* frag = reinterpret_cast<const v8h*>(here) + 4 * NB * kWave + lane;
+      total += part_sum;
+
+      least = min(least, __float_as_uint(info.value_least));
+      const bool rough_values = kAsk && rough_weights(__float_as_uint(info.value_factor), least);
+      if (!rough_values) {
+        if (info.value_factor != unit) {
+          const float g = unit * (1.f / info.value_factor);  // powers of two
+          unit = info.value_factor;
 #pragma unroll
-      for (int b2 = 0; b2 < NB; ++b2)
+          for (int b2 = 0; b2 < NB; ++b2)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[b2][r] *= g;
+        }
+        v8h whi[2], wlo[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const v8h hi = frag[(2 * b2 + c) * kWave], lo = frag[(2 * NB + 2 * b2 + c) * kWave];
-          acc[b2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, whi[c], acc[b2], 0, 0, 0);
-          acc[b2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, wlo[c], acc[b2], 0, 0, 0);
-          acc[b2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, whi[c], acc[b2], 0, 0, 0);
+          const float w[8] = {s[8 * c], s[8 * c + 1], s[8 * c + 2], s[8 * c + 3], s[8 * c + 4], s[8 * c + 5], s[8 * c + 6], s[8 * c + 7]};
+          split8(w, whi[c], wlo[c]);
         }
-    } else {
-      if (unit != 1.f) {
+        const v8h* frag = reinterpret_cast<const v8h*>(here) + 4 * NB * kWave + lane;
 #pragma unroll
         for (int b2 = 0; b2 < NB; ++b2)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[b2][r] *= unit;
-        unit = 1.f;
+          for (int c = 0; c < 2; ++c) {
+            const v8h hi = frag[(2 * b2 + c) * kWave], lo = frag[(2 * NB + 2 * b2 + c) * kWave];
+            acc[b2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, whi[c], acc[b2], 0, 0, 0);
+            acc[b2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, wlo[c], acc[b2], 0, 0, 0);
+            acc[b2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, whi[c], acc[b2], 0, 0, 0);
+          }
+      } else {
+        if (unit != 1.f) {
+#pragma unroll
+          for (int b2 = 0; b2 < NB; ++b2)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[b2][r] *= unit;
+          unit = 1.f;
+        }
+#pragma unroll
+        for (int b2 = 0; b2 < NB; ++b2)
+          acc[b2] = fp32_values(v + cache + 32 * b2, p.dim, p.dim - 32 * b2, j0, seq.keys, reach, s, acc[b2]);
+        loads_done();
       }
-      float weights[16], whole_acc[16 * NB];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) weights[r] = s[r];
-#pragma unroll
-      for (int n2 = 0; n2 < 16 * NB; ++n2) whole_acc[n2] = acc[n2 / 16][n2 % 16];
-      if (wild_values<NB>(v + cache, p.dim, j0, seq.keys, reach, weights, whole_acc)) total = NAN;
-#pragma unroll
-      for (int n2 = 0; n2 < 16 * NB; ++n2) acc[n2 / 16][n2 % 16] = whole_acc[n2];
-      loads_done();
     }
-  }
+  };
+  if (smooth) all(std::false_type());
+  else all(std::true_type());
   if (!mine) return;
   total = across_halves(total, plus);
   if (splits == 1) {

@@ -104,3 +104,19 @@ def test_attention_of_large_values_with_small_weights(gpu, batch, length, q_head
         k[:, :, large, 0] -= F(extra)
         args = ([capacity - length] * batch, [length] * batch, 0, 0, 1, 0.125)
         oracle.attention_by_heads(run_attention(q, k, v, *args), q, k, v, *args)
+
+
+@pytest.mark.parametrize("batch,length,q_heads,kv_heads", SPANS)
+@pytest.mark.parametrize("size", [1e2, 1e5, 1e9, 1e18])
+@pytest.mark.parametrize("where", ["q", "k", "both"])
+def test_attention_of_columns_that_do_not_meet(gpu, batch, length, q_heads, kv_heads, size, where):
+    """Columns of q and of k that are `size` times the others meet zeros: scores do not depend on them."""
+    capacity, dim = 300, 64
+    q, k, _ = inputs(93, batch, length, q_heads, kv_heads, dim, capacity)
+    v = away(94, (batch, kv_heads, capacity, dim))
+    if where != "k":
+        q[..., 5], k[..., 5] = F(size), 0
+    if where != "q":
+        k[..., 40], q[..., 40] = F(size), 0
+    args = ([capacity - length] * batch, [length] * batch, 0, 0, 1, 0.3)
+    oracle.attention_by_heads(run_attention(q, k, v, *args), q, k, v, *args)
