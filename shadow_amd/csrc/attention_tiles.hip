@@ -45,7 +45,7 @@ constexpr int kWaveRows = 32;
 struct alignas(16) TileInfo {
   float key_factor;    // 2^-e of the keys
   float key_sum;       // the largest sum of |x| of a key
-  float value_factor;  // 2^-e of the values; NaN: they need fp32 operands
+  float value_factor;  // 2^-e of the values; NaN: they need fp32 operands, infinite: and so does all behind them
   float value_least;   // the largest |value| of the row that has the smallest one, rows of zeros apart
 };
 
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(kBlock) void attention_split_kernel(const float* k,
   if (tid == 0) {
     infos[blockIdx.x].key_factor = power2(-key_lift), infos[blockIdx.x].key_sum = key_sum;
     infos[blockIdx.x].value_least = smallest;
-    if (wild_values) infos[blockIdx.x].value_factor = NAN;
+    if (wild_values) infos[blockIdx.x].value_factor = value_lift < 0 ? INFINITY : NAN;
   }
 
   // [keys hi][keys lo][values hi][values lo], each 32 * kPadded numbers
@@ -403,6 +403,7 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
   const bool smooth = __builtin_amdgcn_ballot_w64(rough_scores(key_sum, key_factor) || rough_weights(most_factor, least_value)) == 0;
   int buffer = 0;
   uint32_t least = __float_as_uint(INFINITY);  // of the tiles so far, in a scalar register
+  bool far = false;                            // sums may be too large to be taken to other units
   const auto all = [&](auto ask_each) {
     constexpr bool kAsk = decltype(ask_each)::value;
     for (int n = from; n < to; ++n) {
@@ -447,7 +448,10 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
       for (int r = 1; r < 16; ++r) m = larger(m, s[r]);
       m = across_halves(m, larger);
       m = m == -INFINITY ? m : m * f;
-      if (__builtin_amdgcn_ballot_w64(m > top + kLag) != 0) {
+      least = min(least, __float_as_uint(info.value_least));
+      far = kAsk && (far || info.value_factor == INFINITY);
+      const bool rough_values = kAsk && (far || rough_weights(__float_as_uint(info.value_factor), least));
+      if (__builtin_amdgcn_ballot_w64(m > (rough_values ? top : top + kLag)) != 0) {
         const float next = larger(m, top);
         const float g = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
         top = next;
@@ -466,8 +470,6 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
       }
       total += part_sum;
 
-      least = min(least, __float_as_uint(info.value_least));
-      const bool rough_values = kAsk && rough_weights(__float_as_uint(info.value_factor), least);
       if (!rough_values) {
         if (info.value_factor != unit) {
           const float g = unit * (1.f / info.value_factor);  // powers of two
@@ -494,13 +496,15 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
             acc[b2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, whi[c], acc[b2], 0, 0, 0);
           }
       } else {
-        if (unit != 1.f) {
+        // weights of up to 1, as the kernel for few rows has them: nothing overflows here that does not there
+        const float g = unit * __builtin_exp2f(-kLift);
+        unit = __builtin_exp2f(kLift);
 #pragma unroll
-          for (int b2 = 0; b2 < NB; ++b2)
+        for (int b2 = 0; b2 < NB; ++b2)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[b2][r] *= unit;
-          unit = 1.f;
-        }
+          for (int r = 0; r < 16; ++r) acc[b2][r] *= g;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= __builtin_exp2f(-kLift);
 #pragma unroll
         for (int b2 = 0; b2 < NB; ++b2)
           acc[b2] = fp32_values(v + cache + 32 * b2, p.dim, p.dim - 32 * b2, j0, seq.keys, reach, s, acc[b2]);
@@ -540,12 +544,12 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
       for (int c = 0; c < 4; ++c) {
         v4f o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = acc[n][4 * c + e] * unit;
+        for (int e = 0; e < 4; ++e) o[e] = acc[n][4 * c + e] * (unit * __builtin_exp2f(-kLift));
         *reinterpret_cast<v4f*>(sums + slot * kPadded + 32 * n + 8 * c + 4 * half) = o;
       }
     if (half == 0) {
       sums[slots * kPadded + 2 * slot] = top;
-      sums[slots * kPadded + 2 * slot + 1] = total;
+      sums[slots * kPadded + 2 * slot + 1] = total * __builtin_exp2f(-kLift);
     }
   }
 }

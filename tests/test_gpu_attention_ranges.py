@@ -120,3 +120,26 @@ def test_attention_of_columns_that_do_not_meet(gpu, batch, length, q_heads, kv_h
         k[..., 40], q[..., 40] = F(size), 0
     args = ([capacity - length] * batch, [length] * batch, 0, 0, 1, 0.3)
     oracle.attention_by_heads(run_attention(q, k, v, *args), q, k, v, *args)
+
+
+@pytest.mark.parametrize("batch,length,q_heads,kv_heads", SPANS)
+@pytest.mark.parametrize("size", [1e30, 1e33, 1e35, 1e36])
+def test_attention_of_large_finite_values_and_keys(gpu, batch, length, q_heads, kv_heads, size):
+    """Some seen values, then some seen keys, near the end of fp32's range; scores and results are within it."""
+    capacity, dim = 250, 64
+    q, k, _ = inputs(97, batch, length, q_heads, kv_heads, dim, capacity)
+    args = ([capacity - length] * batch, [length] * batch, 0, 0, 1, 0.125)
+    v = away(98, (batch, kv_heads, capacity, dim))
+    v[:, :, 3::40] *= F(size)
+    v[:, :, 100:110] *= F(1e-9)
+    y = run_attention(q, k, v, *args)
+    assert np.isfinite(y).all()
+    oracle.attention_by_heads(y, q, k, v, *args, what="large values")
+    v = away(99, (batch, kv_heads, capacity, dim))
+    k[:, :, 5::50] *= F(size)
+    q *= F(1e-4)
+    for scale, what in ((1e-33, "one key or none"), (1e-2, "one key")):
+        args = args[:5] + (scale,)
+        y = run_attention(q, k, v, *args)
+        assert np.isfinite(y).all()
+        oracle.attention_by_heads(y, q, k, v, *args, what="large keys, " + what)
