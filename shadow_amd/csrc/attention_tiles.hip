@@ -18,7 +18,7 @@
 // contraction may take the keys in any order and the values are stored in that order.
 //
 // A tile is left to the fp32 instruction, from the caches themselves, where a power of two for the whole tile or row
-// would cost precision: where that shows in the scores (rough_keys), where its values' rows and columns differ in size (value_factor),
+// would cost precision: where that shows in the scores (loss), where its values' rows and columns differ in size (value_factor),
 // where values in front of it were far smaller than its own (rough_values), or where something in it is not
 // finite.  So a row that does not see (or hardly weighs) an outlier, and a column that has none, does not suffer from it.
 //
@@ -391,16 +391,16 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
     for (int r = 0; r < 16; ++r) acc[n][r] = 0.f;
   float top = -INFINITY, total = 0.f, unit = 1.f;  // acc is in units of `unit`, a tile's value_factor
 
-  // What the second parts of keys and rows round away, up to 2^-38 of a row's and of a tile's largest number, adds up to 2^-38 of
-  // this in a score; it stays below 2^-22, whatever the scores (in powers of two) are.  Scores of thousands go through fp32, and so
-  // does a tile that holds something that is not finite.
-  const auto rough_scores = [&](float sum, float factor) { return !(wave_most * sum + wave_sum * (factor * 0x1p14f) <= 0x1p16f); };
+  // What the second parts of keys and rows round away, up to 2^-38 of a row's and of a tile's largest number, adds up to this in a
+  // score.  It has to stay below 2^-22, or below 2^-22 of the row's largest score, where fp32 sums are no better: else, and where
+  // something is not finite, the tile's scores are fp32 products.
+  const auto loss = [&](float sum, float factor) { return (wave_most * sum + wave_sum * (factor * 0x1p14f)) * 0x1p-38f; };
   // Values of a tile, less than 2^14 times their factor, are up to 2^12 times the least row's, or need fp32 weights; so does a
   // factor that is a NaN.
   const auto rough_weights = [](uint32_t factor, uint32_t least) { return factor + (2u << 23) > least; };
   for (int step = 1; step < kWave; step <<= 1) least_value = min(least_value, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least_value), step)));
   // Mostly nothing is rough: a loop that does not ask (for NB of 8 the other one has no room for its registers).
-  const bool smooth = __builtin_amdgcn_ballot_w64(rough_scores(key_sum, key_factor) || rough_weights(most_factor, least_value)) == 0;
+  const bool smooth = __builtin_amdgcn_ballot_w64(!(loss(key_sum, key_factor) <= 0x1p-22f) || rough_weights(most_factor, least_value)) == 0;
   int buffer = 0;
   uint32_t least = __float_as_uint(INFINITY);  // of the tiles so far, in a scalar register
   bool far = false;                            // sums may be too large to be taken to other units
@@ -419,35 +419,47 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
       if (!(j0 < wave_b.first || (j0 < wave_b.hi && j0 + kTile > wave_a.lo))) continue;
 
       v16f s;
+      float f, m;
+      const auto score = [&](bool fp32) {
+        if (!fp32) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = 0.f;
-      float f;
-      const bool rough_keys = kAsk && rough_scores(info.key_sum, info.key_factor);
-      if (!rough_keys) {
-        const v8h* frag = reinterpret_cast<const v8h*>(here) + lane;
+          for (int r = 0; r < 16; ++r) s[r] = 0.f;
+          const v8h* frag = reinterpret_cast<const v8h*>(here) + lane;
 #pragma unroll
-        for (int c = 0; c < 2 * NB; ++c) {
-          const v8h hi = frag[c * kWave], lo = frag[(2 * NB + c) * kWave];
-          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qhi[c], s, 0, 0, 0);
-          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qlo[c], s, 0, 0, 0);
-          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, qhi[c], s, 0, 0, 0);
+          for (int c = 0; c < 2 * NB; ++c) {
+            const v8h hi = frag[c * kWave], lo = frag[(2 * NB + c) * kWave];
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qhi[c], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, qlo[c], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, qhi[c], s, 0, 0, 0);
+          }
+          f = __builtin_fmaxf(__builtin_fminf(row_factor * info.key_factor, 0x1p127f), 0x1p-126f);  // neither 0 nor infinite
+        } else {
+          s = fp32_scores<NB>(k + cache + static_cast<uint64_t>(min(j0 + i, p.capacity - 1)) * p.dim, q + at, p.dim, p.scale * kLog2e);
+          f = 1.f;
+          loads_done();
         }
-        f = __builtin_fmaxf(__builtin_fminf(row_factor * info.key_factor, 0x1p127f), 0x1p-126f);  // neither 0 nor infinite
+        if (!((j0 + kTile <= wave_a.first) || (j0 >= wave_b.lo && j0 + kTile <= wave_a.hi))) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!sees(reach, j0 + 8 * (r / 4) + 4 * half + r % 4)) s[r] = -INFINITY;
+        }
+        m = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) m = larger(m, s[r]);
+        m = across_halves(m, larger);
+        m = m == -INFINITY ? m : m * f;
+      };
+      if constexpr (kAsk) {
+        const float lost = loss(info.key_sum, info.key_factor);
+        bool fp32 = !(lost < INFINITY);
+        if (!fp32) {
+          score(false);
+          fp32 = __builtin_amdgcn_ballot_w64(mine && lost > 0x1p-22f * larger(1.f, __builtin_fabsf(m))) != 0;
+        }
+        if (fp32) score(true);
       } else {
-        s = fp32_scores<NB>(k + cache + static_cast<uint64_t>(min(j0 + i, p.capacity - 1)) * p.dim, q + at, p.dim, p.scale * kLog2e);
-        f = 1.f;
-        loads_done();
+        score(false);
       }
-      if (!((j0 + kTile <= wave_a.first) || (j0 >= wave_b.lo && j0 + kTile <= wave_a.hi))) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!sees(reach, j0 + 8 * (r / 4) + 4 * half + r % 4)) s[r] = -INFINITY;
-      }
-      float m = s[0];
-#pragma unroll
-      for (int r = 1; r < 16; ++r) m = larger(m, s[r]);
-      m = across_halves(m, larger);
-      m = m == -INFINITY ? m : m * f;
       least = min(least, __float_as_uint(info.value_least));
       far = kAsk && (far || info.value_factor == INFINITY);
       const bool rough_values = kAsk && (far || rough_weights(__float_as_uint(info.value_factor), least));
@@ -512,7 +524,7 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
       }
     }
   };
-  if (smooth) all(std::false_type());
+  if (__builtin_expect(smooth, 1)) all(std::false_type());
   else all(std::true_type());
   if (!mine) return;
   total = across_halves(total, plus);

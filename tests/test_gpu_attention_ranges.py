@@ -89,6 +89,19 @@ def test_attention_of_a_column_far_larger_than_the_others(gpu, batch, length, q_
 
 
 @pytest.mark.parametrize("batch,length,q_heads,kv_heads", SPANS)
+@pytest.mark.parametrize("dim,size", [(64, 20), (128, 40), (160, 300)])
+def test_attention_of_scores_of_thousands(gpu, batch, length, q_heads, kv_heads, dim, size):
+    """Rows and keys of 20 to 300 standard deviations: a key takes all the weight, or two share it."""
+    capacity = 300
+    q, k, _ = inputs(106, batch, length, q_heads, kv_heads, dim, capacity)
+    v = away(107, (batch, kv_heads, capacity, dim))
+    q, k = q * F(size), k * F(size)
+    k[:, :, 1::2] = k[:, :, ::2] + normal(108, k[:, :, ::2].shape, 0.1 / size)
+    args = ([capacity - length] * batch, [length] * batch, 0, 0, 1, dim ** -0.5)
+    oracle.attention_by_heads(run_attention(q, k, v, *args), q, k, v, *args)
+
+
+@pytest.mark.parametrize("batch,length,q_heads,kv_heads", SPANS)
 @pytest.mark.parametrize("size", [30, 1e4, 1e7, 1e9, 1e12])
 @pytest.mark.parametrize("period", [1, 32, 90])
 def test_attention_of_large_values_with_small_weights(gpu, batch, length, q_heads, kv_heads, size, period):
