@@ -230,7 +230,7 @@ __global__ __launch_bounds__(kRowsWaves * kWave, NB <= 2 ? 2 : 1) void attention
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc[n][c] = f == 0.f ? v4f{0.f, 0.f, 0.f, 0.f} : acc[n][c] * f;
+    for (int c = 0; c < 4; ++c) acc[n][c] *= f;  // what is not finite stays so, however little it weighs
   if (g == 0) totals[wave][i] = total;
 #pragma unroll
   for (int half = kRowsWaves / 2; half >= 1; half /= 2) {
@@ -322,11 +322,11 @@ __global__ __launch_bounds__(kWave) void attention_join_kernel(const float* sums
   for (uint32_t s0 = 0;;) {
 #pragma unroll
     for (int s = 0; s < kTurn; ++s) {
-      const float w = s0 + s < splits ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s0 + s)) : 0.f;
-      if (w != 0.f) {  // a part that saw nothing may hold anything
+      if (s0 + s >= splits) break;
+      // a part that saw nothing holds zeros, one that saw something that is not finite counts with a weight of 0 as well
+      const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s0 + s));
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(o[s][c], w, acc[c]);
-      }
+      for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(o[s][c], w, acc[c]);
     }
     s0 += kTurn;
     if (s0 >= splits) break;

@@ -156,3 +156,16 @@ def test_attention_of_large_finite_values_and_keys(gpu, batch, length, q_heads, 
         y = run_attention(q, k, v, *args)
         assert np.isfinite(y).all()
         oracle.attention_by_heads(y, q, k, v, *args, what="large keys, " + what)
+
+
+@pytest.mark.parametrize("length,capacity", [(1, 64), (3, 64), (1, 700), (3, 3000), (70, 300), (200, 2000)])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_attention_of_values_that_are_not_finite_and_weigh_nothing(gpu, length, capacity, bad):
+    """A seen value that is not finite shows in its column, however small its weight: also where a wave, or a part of the keys,
+    has weights of e^-480 and nothing else."""
+    q, k, v = inputs(101, 1, length, 4, 2, 64, capacity)
+    q[..., 0], k[..., 0] = 8, 0
+    k[:, :, :capacity // 4, 0] = -60
+    v[:, :, 5, 3] = bad
+    y = run_attention(q, k, v, [capacity - length], [length], 0, 0, 1, 1.0)
+    assert not np.isfinite(y[..., 3]).any()
