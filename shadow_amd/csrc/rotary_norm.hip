@@ -44,6 +44,11 @@ SHDW_DEVICE void turn(int64_t position, float frequency, float& c, float& s) {
   sincospif(rest + rest, &s, &c);
 }
 
+// Whether a mean of squares (and eps) in fp32 is one that nothing was lost in: squares of less than 2^-126 are, and so is a sum
+// of more than fp32 holds.  Heads of such sizes, or of zeros with an eps as small, take their mean in fp64.
+SHDW_DEVICE bool exact_mean(float mean) { return mean >= 0x1p-90f && mean < INFINITY; }
+SHDW_DEVICE double norm_factor(double sum, const RotaryArgs& p) { return 1.0 / __builtin_sqrt(sum / p.dim + static_cast<double>(p.eps)); }
+
 // Where head h of token (b, t) goes; nullptr where nothing is written.
 SHDW_DEVICE float* rotary_target(const RotaryArgs& p, float* q, float* k, float* v, uint32_t b, uint32_t t, uint32_t h,
                                  int64_t position) {
@@ -146,7 +151,18 @@ __global__ __launch_bounds__(kBlock) void rotary_heads_kernel(const float* x, fl
         sum = across_head<LANES>(sum);
         const float mean = __builtin_fmaf(sum, p.inv_dim, p.eps), f = 1.f / __builtin_sqrtf(mean);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) y[c] = e[n][c] * f * (is_q ? q_scale[c] : k_scale[c]);
+        for (int c = 0; c < 4; ++c) y[c] = e[n][c] * f;
+        if (__builtin_amdgcn_ballot_w64(!exact_mean(mean) && h < heads && !is_v) != 0) {
+          double wide = 0.0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) wide += static_cast<double>(e[n][c]) * e[n][c];
+          for (int step = 1; step < LANES; step <<= 1) wide += __shfl_xor(wide, step);
+          const double factor = norm_factor(wide, p);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) y[c] = exact_mean(mean) ? y[c] : static_cast<float>(e[n][c] * factor);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) y[c] *= is_q ? q_scale[c] : k_scale[c];
       }
       if (MODE != 0) {
         v4f o;
@@ -200,7 +216,19 @@ __global__ __launch_bounds__(kBlock) void rotary_norm_kernel(const float* x, flo
     sum = __builtin_fmaf(e, e, sum);
   }
   for (int step = 1; step < kWave; step <<= 1) sum += __shfl_xor(sum, step);
-  const float factor = p.normalize ? 1.f / __builtin_sqrtf(__builtin_fmaf(sum, p.inv_dim, p.eps)) : 1.f;
+  float factor = 1.f;
+  if (p.normalize) {
+    const float mean = __builtin_fmaf(sum, p.inv_dim, p.eps);
+    if (exact_mean(mean)) {
+      factor = 1.f / __builtin_sqrtf(mean);
+    } else {
+      double wide = 0.0;
+      for (int d = lane; d < dim; d += kWave) wide += static_cast<double>(head[d]) * head[d];
+      for (int step = 1; step < kWave; step <<= 1) wide += __shfl_xor(wide, step);
+      const double f = norm_factor(wide, p);
+      for (int d = lane; d < dim; d += kWave) head[d] = static_cast<float>(head[d] * f);
+    }
+  }
   const float* scale = !p.normalize ? nullptr : h < static_cast<uint32_t>(p.q_heads) ? p.q_scale : p.k_scale;
   const int half = p.rotary / 2;
   const auto value = [&](int d) { return scale ? head[d] * factor * scale[d] : head[d] * factor; };

@@ -5,7 +5,7 @@ import pytest
 
 from tests import sequence_oracle as oracle
 from tests.helpers import normal, rng
-from tests.test_gpu_attention_layer import inputs, run_attention, run_connected4, weights
+from tests.test_gpu_attention_layer import check_rotary_norm, inputs, run_attention, run_connected4, run_rotary_norm, weights
 
 pytestmark = pytest.mark.gpu
 F = np.float32
@@ -169,3 +169,16 @@ def test_attention_of_values_that_are_not_finite_and_weigh_nothing(gpu, length, 
     v[:, :, 5, 3] = bad
     y = run_attention(q, k, v, [capacity - length], [length], 0, 0, 1, 1.0)
     assert not np.isfinite(y[..., 3]).any()
+
+
+@pytest.mark.parametrize("dim,rotary,interleaved", [(64, 64, 0), (128, 64, 1), (256, 0, 0), (80, 36, 0), (65, 30, 1)])
+@pytest.mark.parametrize("size", [3e38, 1e25, 1e19, 1e-12, 1e-19, 1e-25, 1e-37])
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-6])
+def test_rotary_norm_of_heads_at_the_ends_of_the_range(gpu, dim, rotary, interleaved, size, eps):
+    """Squares may leave fp32's range where the heads and their norms are within it."""
+    x = (away(103, (2, 5, 8, dim)) / F(1.5) * F(size)).astype(F)
+    x[0, 1], x[1, 2, 3] = normal(104, (8, dim)), 0 if eps else 1
+    scale = (1 + normal(105, dim, 0.1)).astype(F)
+    frequency = np.linspace(1, 0.01, rotary // 2).astype(F)
+    args = (4, 2, rotary, interleaved, 1, eps, scale, scale, frequency, [4, 9], None, 20)
+    check_rotary_norm(run_rotary_norm(x, *args), x, *args)
