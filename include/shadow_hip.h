@@ -519,7 +519,9 @@ int shdw_hip_rotary_norm(int batch, int length, int q_heads, int kv_heads, int h
  * A query that sees nothing gives zeros; rows of y of queries that do not count stay as they
  * were.  Keys and values that a query does not see may hold anything, the result's bound does not
  * depend on it (its last bits may: tiles that hold something far off go through other
- * instructions); one that it sees and that is not finite leaves its row of y not finite.
+ * instructions).  A value that it sees and that is not finite leaves its column of the row not
+ * finite, however small its weight, and may leave the whole row so; a key that makes a score NaN or +inf
+ * leaves the row not finite, one that makes it -inf has weight 0.
  * head_dim <= 256; up to 2^30 rows of q and rows of a cache.
  * y may not overlap q, k or v.  `workspace` holds at least
  * shdw_hip_window_attention_workspace_bytes(...) bytes, 16-byte aligned (0 bytes: it may be

@@ -171,6 +171,26 @@ def test_attention_of_values_that_are_not_finite_and_weigh_nothing(gpu, length, 
     assert not np.isfinite(y[..., 3]).any()
 
 
+@pytest.mark.parametrize("batch,length,q_heads,kv_heads", SPANS)
+def test_attention_of_keys_that_are_not_finite(gpu, batch, length, q_heads, kv_heads):
+    """A key that makes a score +inf or NaN leaves its row not finite, one that makes it -inf has weight 0."""
+    capacity, dim = 300, 64
+    q, k, v = inputs(102, batch, length, q_heads, kv_heads, dim, capacity)
+    q[..., 7] = np.where(np.arange(q_heads) % 2, 1, -1) * np.abs(q[..., 7])
+    args = ([capacity - length] * batch, [length] * batch, 0, 0, 1, 0.125)
+    gone = ([capacity - length - 1] * batch,) + args[1:]
+    for bad, hurt in ((np.inf, 1), (-np.inf, 0)):
+        k[:, :, 9, 7] = bad
+        y = run_attention(q, k, v, *args)
+        for h in range(q_heads):
+            if h % 2 == hurt:
+                assert not np.isfinite(y[:, :, h]).any()
+            else:  # as if the key were not there
+                oracle.attention_by_heads(y, q, np.delete(k, 9, 2), np.delete(v, 9, 2), *gone, pairs=[(b, h) for b in range(batch)])
+    k[:, :, 9, 7] = np.nan
+    assert not np.isfinite(run_attention(q, k, v, *args)).any()
+
+
 @pytest.mark.parametrize("dim,rotary,interleaved", [(64, 64, 0), (128, 64, 1), (256, 0, 0), (80, 36, 0), (65, 30, 1)])
 @pytest.mark.parametrize("size", [3e38, 1e25, 1e19, 1e-12, 1e-19, 1e-25, 1e-37])
 @pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-6])
