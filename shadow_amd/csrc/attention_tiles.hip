@@ -528,7 +528,7 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
   else all(std::true_type());
   if (!mine) return;
   total = across_halves(total, plus);
-  if (splits == 1) {
+  if (WAVES == 8 || splits == 1) {
     const bool empty = sees_nothing(reach);
     const float g = unit / total;
 #pragma unroll
@@ -607,7 +607,8 @@ static int launch_tiles_of(const TilesPlan& plan, const float* q, const float* k
       q, k, v, y, parts, infos, sums, plan.tiles, make_fastdiv(plan.heads), make_fastdiv(plan.splits), plan.blocks, p);
   if (int rc = launch_status()) return rc;
   if (plan.splits == 1) return SHDW_OK;
-  return join_parts(sums, y, plan.splits, plan.blocks, WAVES == 8 ? 8 : 7, plan.padded, plan.heads, p, st);
+  static_assert(WAVES == 4 || WAVES == 8, "eight waves, whose workgroups fill the chip, have one part");
+  return join_parts(sums, y, plan.splits, plan.blocks, 7, plan.padded, plan.heads, p, st);
 }
 
 int launch_tiles(const TilesPlan& plan, const float* q, const float* k, const float* v, float* y, void* workspace,
