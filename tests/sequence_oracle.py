@@ -147,3 +147,27 @@ def attention_by_heads(y, q, k, v, starts, lengths, window, sinks, causal, scale
         keys = min(max(int(starts[b]) + n, 0), capacity)
         want, bound = attention_of_head(q[b, :n, h], k[b, h // group], v[b, h // group], int(starts[b]), keys, window, sinks, causal, scale)
         assert_within(y[b, :n, h], want, bound, "%s, head %d of sequence %d" % (what, h, b))
+
+
+def whole_connected4(n_in):
+    """What the result of `n_in` products of random signs may be off by on the whole, 2-norm over 2-norm: operands of 22 bits,
+    and the sums' roundings, which do not line up: twice the square root of their number, the numbers summed being
+    up to twice the result's size."""
+    return 2.0 ** -22 + 2 * HALF * np.sqrt(32 + n_in / 32 + 6)
+
+
+def whole_attention(dim, keys):
+    """The same for attention on numbers of size 1 and scores of size 1: a score's products and sum, an exponential of four
+    half steps, two operands of 22 bits, the sum over the keys."""
+    return 2 * 2.0 ** -22 + 4 * HALF + HALF * (np.sqrt(dim) + 2 * np.sqrt(32 + keys / 16))
+
+
+def assert_close_on_the_whole(got, want, allowed, what=""):
+    """2-norm of the error over the result's, for all of it and for every row (the last axis and what is in front of it
+    apart), where a row may be off by four times that."""
+    got, want = np.asarray(got, np.float64).reshape(-1, np.shape(want)[-1]), np.asarray(want, np.float64).reshape(-1, np.shape(want)[-1])
+    off, size = np.linalg.norm(got - want, axis=1), np.linalg.norm(want, axis=1)
+    assert np.linalg.norm(off) <= allowed * np.linalg.norm(size), "%s: %.3g on the whole, allowed %.3g" % (
+        what, np.linalg.norm(off) / np.linalg.norm(size), allowed)
+    worst = np.argmax(off / np.maximum(size, 1e-300))
+    assert (off <= 4 * allowed * size).all(), "%s: row %d off by %.3g, allowed %.3g" % (what, worst, off[worst] / size[worst], 4 * allowed)
