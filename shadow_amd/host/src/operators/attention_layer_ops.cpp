@@ -35,7 +35,14 @@ class Inputs {
     CHECK_EQ(blob->count(), count) << op_->name() << ": " << what;
     return blob->data<int>();
   }
-  void done() const { CHECK_EQ(at_, inputs_.size()) << op_->name() << ": inputs left over"; }
+  // No input may be an output: its memory may go when that one gets its shape.
+  void done(const Blobs& outputs) const {
+    CHECK_EQ(at_, inputs_.size()) << op_->name() << ": inputs left over";
+    for (const auto& output : outputs) {
+      CHECK(output->data_type() == DataType::kF32) << op_->name() << ": outputs are float blobs";
+      for (const auto& input : inputs_) CHECK_NE(input, output) << op_->name() << ": an output is an input";
+    }
+  }
 
  private:
   const Operator* op_;
@@ -82,9 +89,8 @@ class Connected4Op : public Operator {
     const float* steps = in.floats(true, out * groups, "steps");
     const float* lows = in.floats(has_lows_, out * groups, "lows");
     const float* bias = in.floats(has_bias_, out, "bias");
-    in.done();
+    in.done(outputs);
     auto& output = outputs[0];
-    CHECK_NE(x, output);
     VecInt shape(x->shape().begin(), x->shape().begin() + axis);
     shape.push_back(out);
     output->reshape(countable(shape, name()));
@@ -137,8 +143,7 @@ class RotaryNormOp : public Operator {
     const float* k_scale = in.floats(has_scale_, shape.head_dim, "k_scale");
     const int* starts = in.ints(has_starts_, shape.batch, "starts");
     const int* lengths = in.ints(has_lengths_, shape.batch, "lengths");
-    in.done();
-    for (const auto& output : outputs) CHECK_NE(x, output);
+    in.done(outputs);
     outputs[0]->reshape(countable({shape.batch, shape.length, shape.q_heads, shape.head_dim}, name()));
     const VecInt cache = countable(
         {shape.batch, shape.kv_heads, shape.capacity > 0 ? shape.capacity : shape.length, shape.head_dim}, name());
@@ -191,11 +196,8 @@ class WindowAttentionOp : public Operator {
                                                 q->shape(3), k->shape(2), window_,     sinks_};
     const int* starts = in.ints(has_starts_, shape.batch, "starts");
     const int* lengths = in.ints(has_lengths_, shape.batch, "lengths");
-    in.done();
+    in.done(outputs);
     auto& output = outputs[0];
-    CHECK_NE(q, output);
-    CHECK_NE(k, output);
-    CHECK_NE(v, output);
     output->reshape(q->shape());
     const float scale = has_scale_ ? scale_ : 1.f / std::sqrt(static_cast<float>(shape.head_dim));
     Vision::WindowAttention<DeviceType::kGPU, float>(q->data<float>(), k->data<float>(), v->data<float>(), shape, causal_, scale,

@@ -172,3 +172,29 @@ def test_operator_refusals(gpu):
         assert ws.blob_shape("y1") == [2, 3, 8] and ws.blob_shape("y3") == [2, 1, 3, 8] and ws.blob_shape("y5") == [2, 3, 4, 8]
         want, bound = oracle.window_attention(ws.get_blob("q"), ws.get_blob("k"), ws.get_blob("k"), [0, 0], [3, 3], 0, 0, 1, 8 ** -0.5)
         oracle.assert_within(ws.get_blob("y5"), want, bound, "attention")
+
+
+def test_operators_refuse_an_output_that_is_an_input(gpu):
+    """Every input, not the first alone: what an output's new shape frees would still be read."""
+    with Workspace() as ws:
+        ws.set_blob("x", normal(1, (2, 3, 32)))
+        ws.set_blob("codes", np.zeros((8, 4), np.int32), "int32")
+        for name, size in (("steps", 8), ("lows", 8), ("bias", 8), ("frequency", 4), ("q_scale", 8), ("k_scale", 8)):
+            ws.set_blob(name, np.ones((8, 1) if size == 8 and name in ("steps", "lows") else size, F))
+        for name in ("starts", "lengths"):
+            ws.set_blob(name, np.ones(2, np.int32), "int32")
+        for name, heads in (("q", 4), ("k", 2), ("v", 2)):
+            ws.set_blob(name, normal(2, (2, 3, 4, 8) if name == "q" else (2, heads, 5, 8)))
+        both = {"has_starts": 1, "has_lengths": 1}
+        connected = ["x", "codes", "steps", "lows", "bias"]
+        rotary = ["x", "frequency", "q_scale", "k_scale", "starts", "lengths"]
+        attention = ["q", "k", "v", "starts", "lengths"]
+        heads = {"q_heads": 2, "kv_heads": 1, "head_dim": 8, "has_scale": 1}
+        cases = [("Connected4", connected, [n], {"group": 32, "has_lows": 1, "has_bias": 1}) for n in connected]
+        cases += [("RotaryNorm", rotary, [n if i == at else "o%d" % i for i in range(3)], dict(heads, **both))
+                  for n in rotary for at in range(3)]
+        cases += [("WindowAttention", attention, [n], both) for n in attention]
+        for typ, bottoms, tops, args in cases:
+            with pytest.raises(ShadowError) as e:
+                ws.create_op(typ, bottoms, tops, args).run()
+            assert "output" in str(e.value), (typ, tops, str(e.value))
