@@ -137,7 +137,8 @@ class RotaryNormOp : public Operator {
     CHECK_GE(x->num_axes(), 3);
     auto shape = shape_;
     shape.batch = x->shape(0), shape.length = x->shape(1);
-    CHECK_EQ(x->count(2), (shape.q_heads + 2 * shape.kv_heads) * shape.head_dim);
+    CHECK_EQ(static_cast<long long>(x->count(2)),
+             (static_cast<long long>(shape.q_heads) + 2LL * shape.kv_heads) * shape.head_dim) << name() << ": values of a token";
     const float* frequency = in.floats(shape.rotary_dim > 0, shape.rotary_dim / 2, "frequency");
     const float* q_scale = in.floats(has_scale_, shape.head_dim, "q_scale");
     const float* k_scale = in.floats(has_scale_, shape.head_dim, "k_scale");

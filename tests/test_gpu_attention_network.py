@@ -198,3 +198,7 @@ def test_operators_refuse_an_output_that_is_an_input(gpu):
             with pytest.raises(ShadowError) as e:
                 ws.create_op(typ, bottoms, tops, args).run()
             assert "output" in str(e.value), (typ, tops, str(e.value))
+        with pytest.raises(ShadowError) as e:  # 2^32 + 4 heads are not 4
+            ws.create_op("RotaryNorm", ["x", "frequency"], ["a", "b", "c"],
+                         {"q_heads": 2 ** 31 - 2, "kv_heads": 2 ** 30 + 3, "head_dim": 8, "rotary_dim": 8}).run()
+        assert "values of a token" in str(e.value)
