@@ -920,15 +920,14 @@ static int launch_few_of(const float* x, const char* parts, const float* factors
 template <int GROUP_WORDS, bool LOWS>
 static int launch_few(const float* x, const uint32_t* codes, float* y, void* workspace, const Connected4Args& p, hipStream_t st) {
   const FewPlan f = plan_few(p.rows, p.words * 8, GROUP_WORDS * 8);
-  // Up to 8 rows: one tile of outputs a workgroup, two where that still fills the chip twice: 16384 outputs for four rows 14.8 us with two
-  // and 17.7 with one, 6144 for one row 9.1 and 8.3.  More rows: as many of one, two and four as leave a workgroup for
+  // One row: one tile of outputs a workgroup (32000 outputs 17.0 us, 18.1 with two, 8192 7.0 and 7.2).  Up to 8 rows: one, or two where
+  // that still fills the chip twice: 16384 outputs for four rows 16.6 us with two and 17.9 with one, for eight 16.6 and 20.0; 8192
+  // for four 10.4 and 9.8, for eight 11.4 and 11.5.  More rows: as many of one, two and four as leave a workgroup for
   // each compute unit, since each reads all of x: 16384 outputs for 16 rows 19.5 us with four, 23 with two, 26.5 with one; 4096 for 32 rows
   // 13.2, 10.1 and 11.9.
   const auto wide = [&](uint32_t outputs) { return (p.out + outputs - 1) / outputs * f.sets >= 256; };
   const bool two = p.out >= 16 * 512;
-  if (f.own)
-    return two ? launch_few_of<OneRow<GROUP_WORDS, LOWS>, GROUP_WORDS, 2, LOWS>(x, nullptr, nullptr, codes, y, f, p, st)
-               : launch_few_of<OneRow<GROUP_WORDS, LOWS>, GROUP_WORDS, 1, LOWS>(x, nullptr, nullptr, codes, y, f, p, st);
+  if (f.own) return launch_few_of<OneRow<GROUP_WORDS, LOWS>, GROUP_WORDS, 1, LOWS>(x, nullptr, nullptr, codes, y, f, p, st);
   char* parts = static_cast<char*>(workspace);
   float* factors = reinterpret_cast<float*>(parts + f.sets * f.set_parts);
   const dim3 grid((f.blocks * kBlockWords + kBlock - 1) / kBlock, p.rows);
@@ -953,7 +952,7 @@ static bool connected4_shape(int rows, int in, int out) {
   return rows >= 0 && out >= 0 && in >= 8 && in % 8 == 0 && static_cast<int64_t>(rows) * out <= INT32_MAX &&
          static_cast<int64_t>(rows) * in <= INT32_MAX;
 }
-// Offsets within a workgroup's 32 outputs have 32 bits, and so have the lanes of a grid.
+// Offsets within a workgroup's up to 64 outputs have 32 bits (64 outputs of 2^26 words are 2^32), and so have the lanes of a grid.
 static bool connected4_extents(int rows, int in, int out) { return rows <= 1 << 26 && in <= 1 << 29 && out <= 1 << 26; }
 static bool connected4_group(int group) { return group == 32 || group == 64 || group == 128; }
 
