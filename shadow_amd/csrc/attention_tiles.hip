@@ -22,10 +22,11 @@
 // where values in front of it were far smaller than its own (rough_values), or where something in it is not
 // finite.  So a row that does not see (or hardly weighs) an outlier, and a column that has none, does not suffer from it.
 //
-// A causal prompt of 4096 tokens, 32 heads of 128 values on 8: 391 us, 137 GFLOP of products or 1.06 PFLOP/s of fp16 ones, what
-// a large library product reaches; the split is 12 us of it.  577 patches that all see each other, 16 images, 12 heads of 64: 96 us,
-// the split 22 (113 MB), rows in and out 12, of the rest a half products.  Pieces of 999 tokens in a window of 512, 12 heads of 80:
-// 57 us, 288 workgroups on 256 compute units, so that some have two.
+// A causal prompt of 4096 tokens, 32 heads of 128 values on 8: 370 us, 137 GFLOP of products or 1.11 PFLOP/s of fp16 ones, what
+// a large library product reaches; the split is 13 us of it.  577 patches that all see each other, 16 images, 12 heads of 64: 95 us,
+// the split 21 (113 MB), rows in and out 12, of the rest a half products.  Pieces of 999 tokens in a window of 512, 12 heads of 80:
+// 53 us, 288 workgroups on 256 compute units, so that some have two.  4096 tokens, 16 heads on 4 of 256: 491, of 160 or 192 values
+// (both have room for 192) 350.  A prompt whose tiles all need fp32 takes ten times as long as one that needs none.
 #include "attention_common.h"
 
 #include "../../include/shadow_hip.h"
@@ -392,15 +393,16 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
   float top = -INFINITY, total = 0.f, unit = 1.f;  // acc is in units of `unit`, a tile's value_factor
 
   // What the second parts of keys and rows round away, up to 2^-38 of a row's and of a tile's largest number, adds up to this in a
-  // score.  It has to stay below 2^-22, or below 2^-22 of the row's largest score, where fp32 sums are no better: else, and where
-  // something is not finite, the tile's scores are fp32 products.
+  // score, every rounding at its worst (a twentieth of it is what is met).  It has to stay below 2^-20, or below 2^-22 of the row's
+  // largest score, where fp32 sums are no better: else, and where something is not finite, the tile's scores are fp32 products.
   const auto loss = [&](float sum, float factor) { return (wave_most * sum + wave_sum * (factor * 0x1p14f)) * 0x1p-38f; };
   // Values of a tile, less than 2^14 times their factor, are up to 2^12 times the least row's, or need fp32 weights; so does a
   // factor that is a NaN.
   const auto rough_weights = [](uint32_t factor, uint32_t least) { return factor + (2u << 23) > least; };
   for (int step = 1; step < kWave; step <<= 1) least_value = min(least_value, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least_value), step)));
-  // Mostly nothing is rough: a loop that does not ask (for NB of 8 the other one has no room for its registers).
-  const bool smooth = __builtin_amdgcn_ballot_w64(!(loss(key_sum, key_factor) <= 0x1p-22f) || rough_weights(most_factor, least_value)) == 0;
+  // Mostly nothing is rough: a loop that does not ask.  Asking in every tile a prompt of 4096 takes 400 us for 370, heads of 256
+  // twice as long, since the calls want registers.
+  const bool smooth = __builtin_amdgcn_ballot_w64(!(loss(key_sum, key_factor) <= 0x1p-20f) || rough_weights(most_factor, least_value)) == 0;
   int buffer = 0;
   uint32_t least = __float_as_uint(INFINITY);  // of the tiles so far, in a scalar register
   bool far = false;                            // sums may be too large to be taken to other units
@@ -451,12 +453,20 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
       };
       if constexpr (kAsk) {
         const float lost = loss(info.key_sum, info.key_factor);
+        const auto rough = [&] { return __builtin_amdgcn_ballot_w64(mine && lost > 0x1p-22f * larger(4.f, __builtin_fabsf(m))) != 0; };
         bool fp32 = !(lost < INFINITY);
-        if (!fp32) {
-          score(false);
-          fp32 = __builtin_amdgcn_ballot_w64(mine && lost > 0x1p-22f * larger(1.f, __builtin_fabsf(m))) != 0;
+        if constexpr (NB != 4) {  // of 4 that spills registers: such tiles among others 891 us for a prompt of 4096, 494 in a loop
+          if (!fp32) {
+            score(false);
+            fp32 = rough();
+          }
+          if (fp32) score(true);
+        } else {
+          for (;; fp32 = true) {
+            score(fp32);
+            if (fp32 || !rough()) break;
+          }
         }
-        if (fp32) score(true);
       } else {
         score(false);
       }
@@ -572,8 +582,8 @@ bool plan_tiles(int batch, int length, int q_heads, int kv_heads, int dim, int c
   const int n = (dim + 31) / 32;
   plan->padded = 32 * (n == 5 ? 6 : n == 7 ? 8 : n);
   // Heads of 128 values: eight waves share a tile of 32 KB where rows fill the chip with them twice over (a causal prompt of
-  // 4096 for 32 heads 391 us against 421 with four), four have less to wait for where they do not (pieces of 999 in a
-  // window of 512 71 against 87).  Shorter heads: four (64 values, 577 patches of 16 images 101 against 141).
+  // 4096 for 32 heads 370 us against 393 with four), four have less to wait for where they do not (pieces of 999 in a
+  // window of 512 66 against 87).  Shorter heads: four (64 values, 577 patches of 16 images 95 against 121).
   plan->waves = plan->padded == 128 && (rows + 255) / 256 * heads >= 512 ? 8 : 4;
   const uint32_t block_rows = kWaveRows * plan->waves;
   const int64_t blocks = (rows + block_rows - 1) / block_rows, items = blocks * heads;
@@ -583,7 +593,8 @@ bool plan_tiles(int batch, int length, int q_heads, int kv_heads, int dim, int c
                                          (static_cast<int64_t>(window) * (causal ? 1 : 2) + length) / kTile + 2);
   tiles = std::max<int64_t>(tiles, 1);
   // parts of the keys, where rows alone do not fill the chip: none with fewer than eight tiles.  Two workgroups for a compute unit:
-  // with one 36 rows over 4000 keys of 8 heads take 36 us (40), for 16 sequences of 1900 keys 92 (82); with four 56 and 93
+  // with one 1000 tokens of 32 heads take 62.8 us (60.5), 16 sequences with 96 rows over 1900 keys 52.3 (50.6); with four the first
+  // 68.1, pieces of 999 in a window of 512 79 (66), and 96 rows over 4000 keys of 8 heads gain 0.3 of 37.6
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / items, tiles / 8, 64}));
   if (!grid_fits(items * splits, plan->waves * kWave) || !grid_fits(heads * tiles, kBlock)) return false;
   plan->blocks = static_cast<uint32_t>(blocks), plan->splits = static_cast<uint32_t>(splits);
