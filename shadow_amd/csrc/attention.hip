@@ -380,8 +380,9 @@ static bool plan_rows(int batch, int length, int q_heads, int kv_heads, int dim,
 }
 
 // Which kernel: from 65 rows of a key head on the keys and values are split for the 16-bit instructions first.  Over 4000 keys of
-// 8 heads: 64 rows 30 us without that and 41 with, 96 rows 61 and 42; 16 sequences of 1900 keys of 64 values: 64 rows 81 and 84,
-// 96 rows 131 and 88.
+// 8 heads: 64 rows 31.5 us without that and 35.6 with, 96 rows 53.8 and 37.6; 16 sequences of 1900 keys of 64 values: 64 rows 45.1
+// and 49.0, 96 rows 69.6 and 50.6.  So a token of 65 or more heads on one key head is split too: 128 heads of 64 over 8000 keys 23,
+// of 128 over 65000 88.
 static bool many_rows(int length, int q_heads, int kv_heads) {
   return static_cast<int64_t>(length) * (q_heads / kv_heads) > 64;
 }

@@ -12,13 +12,13 @@
 // a whole number of 23 bits and a sign in units of a group's power of two, in three digits to the base 256; four rows' digits are
 // the 16 rows of the int8 instruction (one of four is not used), codes are int8 numbers after three instructions for
 // eight, and sums are exact.  Workgroups take 16 or 32 outputs, their eight waves an eighth of `in` each.  Digits of one row
-// every workgroup makes for itself, of more rows a launch of their own does (1.7 us).  4096 x 6144 weights for one row 6.3 us
-// (2.1 TB/s of codes and steps), 4096 x 32000 17.2 (4.0 TB/s), 4096 x 16384 with low ends for four rows 14.7 (2.9 TB/s): what is left
+// every workgroup makes for itself, of more rows a launch of their own does (2.6 us).  4096 x 6144 weights for one row 6.9 us
+// (1.9 TB/s of codes and steps), 4096 x 32000 17.0 (4.1 TB/s), 4096 x 16384 with low ends for four rows 13.6 (3.1 TB/s): what is left
 // is launches, the first loads and the steps, which every output has to itself.
 //
 // More rows, by 16: the same with x split into two fp16 numbers, 22 bits of it, since three digits would
-// be three times the products to scale; 5000 x 4099 weights for 13 rows 13.5 us, of which x, read by every workgroup, is most, 16384 x 4096 with
-// low ends for 16 rows 19.5, for 64 54.0.  A code as fp16: four bits at the bottom of 0x6400 are 1024 + code, in the next
+// be three times the products to scale; 5000 x 4099 weights for 13 rows 14.9 us, of which x, read by every workgroup, is most, 16384 x 4096 with
+// low ends for 16 rows 17.2, for 64 49.1.  A code as fp16: four bits at the bottom of 0x6400 are 1024 + code, in the next
 // four bits 1024 + 16 code, so one AND-OR and one packed subtraction make two operands out of a word (nibbles 0 and 4,
 // 1 and 5, and 2 and 6, 3 and 7 after one shift); the odd nibbles' x is a sixteenth.  (The bits alone are the
 // subnormal code * 2^-24, which the instruction takes, but adds up with an error of 5 10^-6: it aligns products by the
@@ -26,7 +26,7 @@
 //
 // From 80 to some hundred rows on, the fewer the larger the weights: x is split once into the order in which lanes take it, tiles of
 // 128 rows x 128 outputs copy it to LDS,
-// four waves of 64 x 64 unpack the codes in registers.  700 rows on 4096 x 4096 weights 83.8 us, 560 TFLOP/s of fp16 products: 192
+// four waves of 64 x 64 unpack the codes in registers.  700 rows on 4096 x 4096 weights 84.3 us, 557 TFLOP/s of fp16 products: 192
 // tiles are a workgroup for three of four compute units, and LDS, unpacking and products take turns there.  Tiles of 64 rows
 // 86.6, eight waves of 32 x 32 102.
 #include <hip/hip_runtime.h>

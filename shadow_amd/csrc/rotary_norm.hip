@@ -11,7 +11,10 @@
 // the product and the turns are formed in fp64 (a position has 31 bits, a frequency 24), the rest,
 // at most half a turn, goes to fp32 sincospi.
 //
-// Bound by its bytes: two prompts of up to 4096 tokens, 48 heads of 128 values, 61.4 us, 5.2 TB/s (a large copy: 4.8); one token 2.9 us, a launch.
+// Bound by its bytes: two prompts of up to 4096 tokens, 48 heads of 128 values, 63 us, 5.1 TB/s (a large copy: 4.8); one token 3.7 us, a launch.
+// That is heads of up to 256 values and a rotated part that are whole vectors (rotary_heads_kernel).  Any other head takes
+// rotary_norm_kernel, a wave a head, which works the angles out for each and goes through LDS: the same prompts with heads of 126
+// values 282 us, of 128 with 36 of them turned 243, of 512 915.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
