@@ -468,8 +468,11 @@ int shdw_hip_group_norm_ws(int outer_num, int inner_num, float eps, const float*
 /* Three operators that the reference lacks, for the attention half of a transformer's
  * layer: products with 4-bit weights, norms and position rotation of queries and keys
  * on their way into the caches, attention over these.  Their fp32 sums are associated as
- * the kernels find best and multiplications and additions may be fused; results are
- * within a few fp32 roundings of the formulas and the same on every call. */
+ * the kernels find best and multiplications and additions may be fused; results are the same on
+ * every call and within a few fp32 roundings of what the formulas add up: for Connected4 the sum of
+ * |x| (|low| + 15 |step|), for WindowAttention scores as fp32 sums of products and the weighted sum
+ * of |v| in the column (a number of v is off by up to 2^-35 of what is largest among 32 neighbouring keys, unless
+ * that shows in whole rows or columns of them). */
 
 /* Connected4: y [rows][out] = x [rows][in] W^T + bias, weights of four bits in groups of
  * `group` (32, 64 or 128) neighbours along `in`,
@@ -479,7 +482,8 @@ int shdw_hip_group_norm_ws(int outer_num, int inner_num, float eps, const float*
  * [out][ceil(in / group)]; lows == NULL takes -8 * steps (codes 0..15 as -8..7).  bias may
  * be NULL.  `workspace` holds at least shdw_hip_connected4_workspace_bytes(...) bytes,
  * 16-byte aligned (0 bytes: it may be NULL); calls that share one are ordered by the caller.
- * A value of x that is not finite makes its row of y not finite, and no other.  Up to 2^26
+ * A value of x that is not finite makes its row of y not finite, and no other.  y may not overlap
+ * what is read.  Up to 2^26
  * rows and outputs, in up to 2^29, steps and lows of up to 2^90 in size.
  * ref: shadow/operators/connected_op.cpp is the operator with fp32 weights */
 size_t shdw_hip_connected4_workspace_bytes(int rows, int in, int out, int group);
