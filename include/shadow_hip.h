@@ -484,7 +484,7 @@ int shdw_hip_group_norm_ws(int outer_num, int inner_num, float eps, const float*
  * 16-byte aligned (0 bytes: it may be NULL); calls that share one are ordered by the caller.
  * A value of x that is not finite makes its row of y not finite, and no other.  y may not overlap
  * what is read.  Up to 2^26
- * rows and outputs, in up to 2^29, steps and lows of up to 2^90 in size.
+ * rows and outputs, in up to 2^29, steps and lows of up to 2^80 in size.
  * ref: shadow/operators/connected_op.cpp is the operator with fp32 weights */
 size_t shdw_hip_connected4_workspace_bytes(int rows, int in, int out, int group);
 int shdw_hip_connected4(int rows, int in, int out, int group, const float* x, const int* codes,

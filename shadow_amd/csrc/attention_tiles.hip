@@ -366,8 +366,8 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
         m = larger(m, __builtin_fabsf(x[s][e]));
         sum += __builtin_fabsf(x[s][e]);
       }
-    m = across_halves(m, larger);
-    wave_most = mine ? m : 0.f, wave_sum = mine ? across_halves(sum, plus) : 0.f;
+    m = across_halves(m, larger), sum = across_halves(sum, plus);
+    wave_most = mine ? m : 0.f, wave_sum = mine ? sum : 0.f;
     for (int step = 1; step < 32; step <<= 1) {
       wave_most = larger(wave_most, __shfl_xor(wave_most, step));
       wave_sum = larger(wave_sum, __shfl_xor(wave_sum, step));
