@@ -483,11 +483,13 @@ __global__ __launch_bounds__(WAVES * kWave, NB <= 4 ? 2 : 1) void attention_tile
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[b2][r] *= g;
       }
-      const float shift = (top == -INFINITY ? 0.f : top) - kLift;
+      // Scores of 2^22 and more have steps of a half and more: rounded as `top` is they are at most top + kLag, in one step they could
+      // be far above it, and their weights infinite in fp16.  Where nothing is lost they are below 2^18.
+      const float base = top == -INFINITY ? 0.f : top, shift = base - kLift;
       float part_sum = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], f, -shift));
+        s[r] = __builtin_amdgcn_exp2f(kAsk ? (s[r] * f - base) + kLift : __builtin_fmaf(s[r], f, -shift));
         part_sum += s[r];
       }
       total += part_sum;

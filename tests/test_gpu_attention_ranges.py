@@ -102,6 +102,23 @@ def test_attention_of_scores_of_thousands(gpu, batch, length, q_heads, kv_heads,
 
 
 @pytest.mark.parametrize("batch,length,q_heads,kv_heads", SPANS)
+@pytest.mark.parametrize("dim", [64, 128, 160])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e8, 1e9, 1e12])
+def test_attention_of_scores_beyond_units(gpu, batch, length, q_heads, kv_heads, dim, size):
+    """Scores whose steps are units and more: weights are those of rounded scores, results finite and between the seen values."""
+    capacity = 300
+    q, k, _ = inputs(109, batch, length, q_heads, kv_heads, dim, capacity)
+    v = away(110, (batch, kv_heads, capacity, dim))
+    k *= np.exp(np.linspace(0, np.log(size), capacity))[rng(111).permutation(capacity)].astype(F)[:, None]
+    args = ([capacity - length] * batch, [length] * batch, 0, 0, 1, 1.0)
+    y = run_attention(q, k, v, *args)
+    assert np.isfinite(y).all()
+    wide = np.abs(v).max() * (1 + 2.0 ** -18)
+    assert (np.abs(y) <= wide).all()
+    oracle.attention_by_heads(y, q, k, v, *args)
+
+
+@pytest.mark.parametrize("batch,length,q_heads,kv_heads", SPANS)
 @pytest.mark.parametrize("size", [30, 1e4, 1e7, 1e9, 1e12])
 @pytest.mark.parametrize("period", [1, 32, 90])
 def test_attention_of_large_values_with_small_weights(gpu, batch, length, q_heads, kv_heads, size, period):
