@@ -59,12 +59,12 @@ SHDW_DEVICE v8h operand_of(uint32_t word) {
                     (high & 0x00f000f0u) | k1024};
   return __builtin_bit_cast(v8h, bits) - static_cast<_Float16>(1024.f);
 }
-// Eight values of x in the same order, split.
-SHDW_DEVICE void operand_of(const float (&x)[8], float factor, v8h& hi, v8h& lo) {
+// Eight values of x, lifted, in the same order, split.
+SHDW_DEVICE void operand_of(const float (&x)[8], v8h& hi, v8h& lo) {
   constexpr int kNibble[8] = {0, 4, 1, 5, 2, 6, 3, 7};
   float v[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = x[kNibble[e]] * (kNibble[e] % 2 ? factor * 0.0625f : factor);
+  for (int e = 0; e < 8; ++e) v[e] = kNibble[e] % 2 ? x[kNibble[e]] * 0.0625f : x[kNibble[e]];
   split8(v, hi, lo);
 }
 SHDW_DEVICE void load8(const float* p, float (&x)[8]) {
@@ -128,14 +128,14 @@ SHDW_DEVICE Digits digits_of(const float (&v)[8]) {
 #pragma unroll
   for (int c = 0; c < 8; ++c) most = larger_or_nan(most, __builtin_fabsf(v[c]));
   most = across_lanes<GROUP_WORDS>(most, [](float a, float b) { return larger_or_nan(a, b); });
-  // the largest in [2^22, 2^23) / 1.0045: three digits hold up to 127 * 65793 = 2^23 / 1.0039; up to 2^148, in two steps
-  const int e = 22 - max(-126, exponent_of(most * 1.0045f));
-  const float f = power2(min(e, 126)), f2 = power2(max(e - 126, 0));
+  // the largest in [2^22, 2^23) / 1.0045: three digits hold up to 127 * 65793 = 2^23 / 1.0039; up to 2^149, with which
+  // subnormal numbers are whole
+  const int e = 22 - exponent_of(most * 1.0045f);
   uint32_t top[2] = {}, middle[2] = {}, low[2] = {};
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
     // v = 65536 a + 256 b + c, each in -128 .. 127
-    const float scaled = v[c] * f * f2;
+    const float scaled = lifted(v[c], e);
     sum += scaled;
     const int d = static_cast<int>(__builtin_rintf(scaled));
     const int lo = static_cast<int8_t>(d), rest = (d - lo) >> 8, mid = static_cast<int8_t>(rest), hi = (rest - mid) >> 8;
@@ -146,7 +146,7 @@ SHDW_DEVICE Digits digits_of(const float (&v)[8]) {
   }
   Digits d;
   d.top = make_uint2(top[0], top[1]), d.middle = make_uint2(middle[0], middle[1]), d.low = make_uint2(low[0], low[1]);
-  d.factor = most < INFINITY ? __builtin_ldexpf(1.f, -e) : NAN;  // digits hold nothing that is not finite
+  d.factor = most < INFINITY ? lift_undone(e) : NAN;  // digits hold nothing that is not finite
   sum = across_lanes<GROUP_WORDS>(sum, [](float a, float b) { return a + b; });
   d.sum = LOWS ? sum : sum * -8.f;
   return d;
@@ -290,12 +290,15 @@ __global__ __launch_bounds__(kBlock) void connected4_halves_kernel(const float* 
 #pragma unroll
   for (int c = 0; c < 8; ++c) most = larger(most, __builtin_fabsf(v[c]));
   most = across_lanes<GROUP_WORDS>(most, [](float a, float b) { return larger(a, b); });
-  const int e = lift_of(most);
+  const int e = far_lift_of(most);
 #pragma unroll
-  for (int c = 0; c < 8; ++c) sum = __builtin_fmaf(v[c], power2(e), sum);
+  for (int c = 0; c < 8; ++c) {
+    v[c] = lifted(v[c], e);
+    sum += v[c];
+  }
   sum = across_lanes<GROUP_WORDS>(sum, [](float a, float b) { return a + b; });
   v8h hi, lo;
-  operand_of(v, power2(e), hi, lo);
+  operand_of(v, hi, lo);
   int g, t;
   few_place<GROUP_WORDS>(at % kBlockWords, g, t);
   v8h* to = reinterpret_cast<v8h*>(parts + ((((static_cast<uint64_t>(set) * blocks + block) * 4 + t) * 4 + g) * 16 + row) * 32);
@@ -303,7 +306,7 @@ __global__ __launch_bounds__(kBlock) void connected4_halves_kernel(const float* 
   if (at % GROUP_WORDS == 0) {
     const uint64_t groups = static_cast<uint64_t>(blocks) * (kBlockWords / GROUP_WORDS);
     float* out = factors + (set * groups + at / GROUP_WORDS) * 32 + row;
-    out[0] = power2(-e), out[16] = LOWS ? sum : sum * -8.f;
+    out[0] = lift_undone(e), out[16] = LOWS ? sum : sum * -8.f;
   }
 }
 template <int GROUP_WORDS, bool LOWS>
@@ -566,8 +569,8 @@ __global__ __launch_bounds__(kBlock) void connected4_split_kernel(const float* x
       for (int c = 0; c < 8; ++c) most = larger(most, __builtin_fabsf(v[n][c]));
   }
   for (int s = 1; s < 32; s <<= 1) most = larger(most, __shfl_xor(most, s));
-  const int e = lift_of(most);
-  if (blockIdx.y == 0 && lane == 0) undo[row] = power2(-e);
+  const int e = far_lift_of(most);
+  if (blockIdx.y == 0 && lane == 0) undo[row] = lift_undone(e);
   const uint32_t turns = (stages + 3) / 4;  // of 32 words: four stages, whole groups
   const uint32_t from = turns * blockIdx.y / kSplitParts, to = turns * (blockIdx.y + 1) / kSplitParts;
   const uint32_t block = row / 32, r = row % 32;
@@ -588,16 +591,31 @@ __global__ __launch_bounds__(kBlock) void connected4_split_kernel(const float* x
         group_most = larger(group_most, __builtin_fabsf(v[c]));
       }
       group_most = across_lanes<GROUP_WORDS>(group_most, [](float a, float b) { return larger(a, b); });
-      const int lift = group_most == 0.f || group_most >= most * kNear ? e : min(lift_of(group_most), e + kMostLift);
+      const int lift = group_most == 0.f || group_most >= most * kNear ? e : min(far_lift_of(group_most), e + kMostLift);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[c] *= power2(min(e, 126));
+      if (e > 126) {  // rare, like the next: branches, not multiplications for all
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] *= power2(e - 126);
+      }
       // in the units of the products, where they are added to them, else in the row's
 #pragma unroll
-      for (int c = 0; c < 8; ++c) sum = __builtin_fmaf(v[c], power2(LOWS ? e : lift), sum);
+      for (int c = 0; c < 8; ++c) sum += v[c];
+      if (lift != e) {
+        float own_sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          v[c] = lifted(real ? all[n][c] : 0.f, lift);
+          own_sum += v[c];
+        }
+        if (!LOWS) sum = own_sum;
+        own = true;
+      }
       sum = across_lanes<GROUP_WORDS>(sum, [](float a, float b) { return a + b; });
       if (stage >= stages) continue;
-      own = own || lift != e;
       const int word = w % kStageWords;
       v8h hi, lo;
-      operand_of(v, power2(lift), hi, lo);
+      operand_of(v, hi, lo);
       v8h* out = parts + (static_cast<uint64_t>(block) * stages + stage) * (kStageBytes / 16) + stage_product(word) * kWave +
                  stage_lane(word, r);
       out[0] = hi;
@@ -768,7 +786,6 @@ __global__ __launch_bounds__(kBlock, 1) void connected4_many_kernel(const v8h* p
   };
   // two stages are on their way while one is worked on; `from` and `to` are even, a group of 128 is two stages
   constexpr bool kEvery = GROUP_WORDS < 16;  // stage has groups of its own
-  if (from < to) fetch(from, true), fetch(from + 1, true);
   const auto all = [&](auto factors) {
     for (uint32_t stage = from; stage < to; stage += 2) {
       copies_done<kCopies>();
@@ -785,6 +802,7 @@ __global__ __launch_bounds__(kBlock, 1) void connected4_many_kernel(const v8h* p
       work(stage + 1, k, kEvery, true, factors);
     }
   };
+  if (from < to) fetch(from, true), fetch(from + 1, true);
   // Factors of groups, where any of the 128 rows has one: a loop of its own, since looking for them in every group takes 6 % of
   // 700 rows on 4096 x 4096 weights, 11 % with groups of 64.
   if (some != 0) all(std::true_type());

@@ -16,6 +16,11 @@ SHDW_DEVICE float power2(int e) { return __int_as_float((e + 127) << 23); }  // 
 SHDW_DEVICE int exponent_of(float v) { return static_cast<int>((__float_as_uint(v) >> 23) & 255u) - 127; }
 // e such that 2^e times the largest of some numbers is in [2^13, 2^14), as far as 2^e and 2^-e are normal.
 SHDW_DEVICE int lift_of(float largest) { return max(-126, min(126, 13 - exponent_of(largest))); }
+// The same up to 140, which makes subnormal numbers whole multiples of 2^-9: what is lifted by it is multiplied twice, and
+// 2^-e is subnormal too.
+SHDW_DEVICE int far_lift_of(float largest) { return max(-126, 13 - exponent_of(largest)); }
+SHDW_DEVICE float lifted(float v, int e) { return v * power2(min(e, 126)) * power2(max(e - 126, 0)); }
+SHDW_DEVICE float lift_undone(int e) { return __builtin_ldexpf(1.f, -e); }
 SHDW_DEVICE float larger(float a, float b) { return __builtin_fmaxf(a, b); }  // a NaN loses
 SHDW_DEVICE float larger_or_nan(float a, float b) { return b <= a || a != a ? a : b; }
 

@@ -55,11 +55,11 @@ def test_connected4_groups_of_very_different_sizes(gpu, rows, n_in, n_out, group
 
 @pytest.mark.parametrize("rows,n_in,n_out,group", FORMS)
 @pytest.mark.parametrize("lows", [False, True])
-@pytest.mark.parametrize("size", [3e38, 2e35, 1e-37])
+@pytest.mark.parametrize("size", [3e38, 2e35, 1e-37, 1e-40, 1e-43])
 def test_connected4_of_values_at_the_ends_of_the_range(gpu, rows, n_in, n_out, group, lows, size):
     """Sums of code * x and of x may leave fp32's range where x and the result are within it."""
     codes, steps, low = weights(87, n_in, n_out, group, lows)
-    scale = F(1e-6) if size > 1 else F(50)
+    scale = F(1e-6) if size > 1 else F(50 * 1e-37 / size)
     steps *= scale
     if lows:
         low *= scale
