@@ -26,7 +26,7 @@
 //
 // From 80 to some hundred rows on, the fewer the larger the weights: x is split once into the order in which lanes take it, tiles of
 // 128 rows x 128 outputs copy it to LDS,
-// four waves of 64 x 64 unpack the codes in registers.  700 rows on 4096 x 4096 weights 84.3 us, 557 TFLOP/s of fp16 products: 192
+// four waves of 64 x 64 unpack the codes in registers.  700 rows on 4096 x 4096 weights 84 us, 560 TFLOP/s of fp16 products: 192
 // tiles are a workgroup for three of four compute units, and LDS, unpacking and products take turns there.  Tiles of 64 rows
 // 86.6, eight waves of 32 x 32 102.
 #include <hip/hip_runtime.h>
@@ -700,7 +700,7 @@ __global__ __launch_bounds__(kBlock, 1) void connected4_many_kernel(const v8h* p
   };
 
   static_assert(kManyRows / kSplitRows * kSplitParts == kWave, "a lane a word");
-  const uint64_t some = __builtin_amdgcn_ballot_w64(apart[row_tile * kWave + lane] != 0);
+  const uint32_t some = apart[row_tile * kWave + lane];  // asked for in front of the copies, looked at behind the first of them
 
   v16f acc[2][2], run[2][2];  // [32 rows][32 outputs]
 #pragma unroll
@@ -784,7 +784,7 @@ __global__ __launch_bounds__(kBlock, 1) void connected4_many_kernel(const v8h* p
       }
     }
   };
-  // two stages are on their way while one is worked on; `from` and `to` are even, a group of 128 is two stages
+  // two stages are on their way while one is worked on; `from` and `to` are even and differ, a group of 128 is two stages
   constexpr bool kEvery = GROUP_WORDS < 16;  // stage has groups of its own
   const auto all = [&](auto factors) {
     for (uint32_t stage = from; stage < to; stage += 2) {
@@ -802,11 +802,13 @@ __global__ __launch_bounds__(kBlock, 1) void connected4_many_kernel(const v8h* p
       work(stage + 1, k, kEvery, true, factors);
     }
   };
-  if (from < to) fetch(from, true), fetch(from + 1, true);
+  asm volatile("" ::: "memory");
+  fetch(from, true), fetch(from + 1, true);
+  copies_done<kCopies>();
   // Factors of groups, where any of the 128 rows has one: a loop of its own, since looking for them in every group takes 6 % of
   // 700 rows on 4096 x 4096 weights, 11 % with groups of 64.
-  if (some != 0) all(std::true_type());
-  else all(std::false_type());
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(some != 0) == 0, 1)) all(std::false_type());
+  else all(std::true_type());
   // everything is loaded in front of the first store: a load behind one waits for it
   v4f back[2][4];
   float bias[2];
